@@ -55,7 +55,8 @@ enum {
   MI_STATUS_BAD_BATCH_INDEX = 8, /* batch index outside [0, batch_size): skipped */
   MI_STATUS_POOL_OVERFLOW = 16,  /* release would overfill the free list (double free) */
   MI_STATUS_SLOT_FULL = 32,      /* a slot's page table row is full: nothing popped */
-  MI_STATUS_TIMEOUT = 64         /* a bounded device-side wait gave up: results invalid */
+  MI_STATUS_TIMEOUT = 64,        /* a bounded device-side wait gave up: results invalid */
+  MI_STATUS_NO_TOKEN = 128       /* a row of logits without one above -inf: token -1 */
 };
 
 /* Message for the last non-OK return on this thread ("" if none). */
@@ -324,6 +325,36 @@ int mi_silu_mul(const void *gate_up, void *out, int32_t rows, int32_t inter, int
 int mi_proj_small_m(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias,
                     void *y, int64_t ldy, int32_t m, int32_t n, int32_t k, int32_t dtype,
                     int32_t *status, mi_stream_t stream);
+
+/* ---- sampling ----------------------------------------------------------- */
+
+/* One token per row of logits[rows][vocab] (row stride in elements, unit
+ * stride in a row, any element alignment): temperature, top-k, top-p and
+ * min-p with one given random number per row, where the reference samples
+ * with temperature alone (scheduler.py:310-343).
+ *
+ * With w_i = exp((x_i - max x) / T) and the order (x descending, index
+ * ascending): kept are the first top_k tokens; of those the shortest prefix
+ * that holds at least top_p of their mass; of those the ones with
+ * w_i >= min_p (relative to the likeliest token's 1). The first token of the
+ * order is always kept. The result is the first kept token by index whose
+ * running mass exceeds uniform[row] times the kept mass.
+ *   temperature <= 0 (or NaN): the largest logit, lowest index first, filters
+ *     ignored. top_k <= 0 or >= vocab, top_p >= 1 (or NaN), min_p <= 0 (or
+ *     NaN): filter off. uniform is taken into [0, 1) (NaN: 0).
+ *   A NaN logit counts as -inf, and -inf is never chosen; among +inf logits
+ *     the weight is shared equally. A row with nothing above -inf gives -1,
+ *     log-probability -inf and MI_STATUS_NO_TOKEN.
+ * Each setting is per row (a device array of `rows`) or, where the array is
+ * NULL, the scalar after it for all rows. logprob (optional): log-softmax of
+ * the unscaled, unfiltered logits at the token. Deterministic (integer
+ * masses); exact where two masses differ by more than about 2^-44 of the
+ * likeliest token's. vocab <= 262144, no workspace. */
+int mi_sample_tokens(const void *logits, int64_t row_stride, int32_t rows, int32_t vocab,
+                     int32_t dtype, const float *uniform, const float *temperature,
+                     float temperature_all, const int32_t *top_k, int32_t top_k_all,
+                     const float *top_p, float top_p_all, const float *min_p, float min_p_all,
+                     int32_t *out, float *logprob, int32_t *status, mi_stream_t stream);
 
 /* ---- tensor parallelism: fused all-reduce for decode steps --------------- */
 

@@ -1,6 +1,8 @@
 """Tensor -> C-ABI argument helpers (pointers, dtypes, the current stream)."""
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import capi
@@ -25,6 +27,14 @@ def stream_of(t: torch.Tensor) -> int:
     if not t.is_cuda:
         raise capi.MiError("mi_b200 ops need CUDA tensors (no CPU fallback)")
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def on_device_of(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one: launches and kernel
+    attributes go to the current device, whatever the stream's."""
+    if t.device.index is None or t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
 
 
 def need_i32(name: str, t: torch.Tensor, device) -> torch.Tensor:

@@ -20,6 +20,7 @@ ERR_INVALID, ERR_UNSUPPORTED, ERR_WORKSPACE, ERR_CUDA = 1, 2, 3, 4
 STATUS_BITS = {
     1: "OUT_OF_PAGES", 2: "BAD_PAGE", 4: "BAD_POSITION", 8: "BAD_BATCH_INDEX",
     16: "POOL_OVERFLOW", 32: "SLOT_FULL", 64: "TIMEOUT",
+    128: "NO_TOKEN",
 }
 
 
@@ -83,6 +84,8 @@ _SIGS = {
     "mi_silu_mul": ([_c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_p], ctypes.c_int),
     "mi_proj_small_m": ([_c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_i32, _c_i32, _c_i32,
                          _c_i32, _c_p, _c_p], ctypes.c_int),
+    "mi_sample_tokens": ([_c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_p, _c_p, _c_f, _c_p, _c_i32,
+                          _c_p, _c_f, _c_p, _c_f, _c_p, _c_p, _c_p, _c_p], ctypes.c_int),
     "mi_allreduce_add_rmsnorm": ([_c_p, _c_i64, _c_i64, _c_p, _c_i32, _c_i32, _c_p, _c_p, _c_p,
                                  _c_i32, _c_i32, _c_f, _c_i32, _c_p, _c_p], ctypes.c_int),
     "mi_set_peer_wait_limit_ns": ([_c_i64], ctypes.c_int),
