@@ -233,6 +233,54 @@ int mi_paged_prefill(
     mi_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Accumulated attention weights (no counterpart in the reference, whose cache
+ * keeps every token): what mi_kv_evict ranks cached tokens by.
+ *
+ * scores[num_pages][num_kv_heads][page_size] (fp32, one array per layer,
+ * beside the layer's pool): a call adds to each token's entry the softmax
+ * weight the call's queries gave it, summed over the query heads of the KV
+ * head's group. Entries of slots past a request's tokens are not touched. A
+ * page listed twice in one call receives both sums.
+ *
+ * mi_paged_decode_scores: mi_paged_decode (k_new NULL) or
+ * mi_paged_decode_append (k_new given; same coverage, MI_ERR_UNSUPPORTED
+ * otherwise) with the scores accumulated on the way: same out and lse.
+ * rope_positions (optional, with k_new): the RoPE position of each request's
+ * new token, which after an eviction is no longer its slot kv_len - 1.
+ * max_pages: entries of kv_indices. scratch (256-byte aligned,
+ * mi_paged_decode_scores_scratch_size() bytes, contents irrelevant) holds the
+ * logits between two kernels; calls that may overlap on the GPU need their own.
+ *
+ * mi_paged_prefill_scores: the weights given by the last `window` queries of
+ * each request (window <= 0: all of them) of an mi_paged_prefill call with
+ * the same arguments, from the lse it returned ([total_q][num_qo_heads],
+ * natural log; -inf: the row saw nothing). Queries are not read outside the
+ * window.
+ * ------------------------------------------------------------------------- */
+size_t mi_paged_decode_scores_scratch_size(int32_t batch_size, int32_t num_qo_heads,
+                                           int32_t page_size, int64_t max_pages);
+int mi_paged_decode_scores(
+    const void *q, int64_t q_stride_b, int64_t q_stride_h,
+    const void *k_new, int64_t k_stride_b, int64_t k_stride_h,
+    const void *v_new, int64_t v_stride_b, int64_t v_stride_h,
+    const void *rope_cos, const void *rope_sin, int32_t rope_max_pos,
+    const int32_t *rope_positions,
+    void *kv_data, int64_t num_pages, int32_t page_size, int32_t num_kv_heads,
+    int32_t head_dim, int32_t dtype,
+    const int32_t *kv_indptr, const int32_t *kv_indices, int64_t max_pages,
+    const int32_t *kv_last_page_len, int32_t batch_size, int32_t num_qo_heads, float sm_scale,
+    void *out, float *lse, float *scores, void *scratch, size_t scratch_bytes,
+    void *workspace, size_t workspace_bytes, int32_t *status, mi_stream_t stream);
+int mi_paged_prefill_scores(
+    const void *q, int64_t q_stride_n, int64_t q_stride_h,
+    const int32_t *qo_indptr, int32_t total_q,
+    const void *kv_data, int64_t num_pages, int32_t page_size, int32_t num_kv_heads,
+    int32_t head_dim, int32_t dtype,
+    const int32_t *kv_indptr, const int32_t *kv_indices, const int32_t *kv_last_page_len,
+    int32_t batch_size, int32_t num_qo_heads, int32_t causal, int32_t window, float sm_scale,
+    const float *lse, float *scores, int32_t *status, mi_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * (4) Device page pool (replaces PagedKVCache's free list, scheduler.py:168-221)
  *
  * free_ring[num_pages] and pool_ctrl[4] are caller-owned device int32
@@ -278,6 +326,44 @@ int mi_slot_release(int32_t *free_ring, int32_t *pool_ctrl, int32_t num_pages,
                     const int32_t *slots, int32_t n, void *const *layer_pools,
                     int32_t num_layers, int64_t page_bytes, int32_t *status,
                     mi_stream_t stream);
+/* After an eviction (mi_kv_evict): slots[0..n) keep their first keep_pages
+ * pages; the others go to the free list (slot order, then allocation order),
+ * zeroed in every layer, and their scores too (scores: [num_layers]
+ * [num_pages][score_page_elems] fp32, or NULL). keep_pages = 0 retires the
+ * slots as mi_slot_release does. */
+int mi_slot_trim(int32_t *free_ring, int32_t *pool_ctrl, int32_t num_pages,
+                 int32_t *page_table, int32_t *slot_num_pages, int32_t max_slots,
+                 int32_t max_pages_per_slot, const int32_t *slots, int32_t n,
+                 int32_t keep_pages, void *const *layer_pools, int32_t num_layers,
+                 int64_t page_bytes, float *scores, int32_t score_page_elems,
+                 int32_t *status, mi_stream_t stream);
+/* Eviction by accumulated attention weight. Every request of the CSR page
+ * table with more than `budget` tokens is cut to `budget`, in each layer and
+ * KV head by itself: kept are its first `sinks` slots, its last `recent`
+ * slots, and the budget - recent - sinks tokens between them with the largest
+ * scores (equal: the lowest slot; NaN ranks lowest). Afterwards slots
+ * 0..budget-1 hold the kept tokens: one of the first or middle ones below
+ * slot budget - recent stays where it is, the others fill the evicted ones'
+ * slots in order (i-th to i-th), and the recent ones follow in their order.
+ * Scores move along, and are 0 from slot `budget` to the end of the request's
+ * pages. Slots of K and V past the budget keep their contents. The page table
+ * is not changed (kv_last_page_len still counts the old length): the caller
+ * plans with the new length and releases pages with mi_slot_trim.
+ * The layers' pools are layer_pools (device array of pointers, 16-byte
+ * aligned pools) or, where that is NULL, kv_data + layer * kv_layer_stride
+ * elements; scores: [num_layers][num_pages][num_kv_heads][page_size]. kept
+ * (optional): [num_layers][batch][num_kv_heads][budget], the slot each kept
+ * token came from (-1 past a shorter request). max_len: an upper bound of the
+ * requests' lengths (sizes the shared memory; at most 819200 tokens). A longer
+ * request (MI_STATUS_BAD_POSITION) or one with a page outside the pool
+ * (MI_STATUS_BAD_PAGE) is left as it is, kept = -1. A page may be listed once
+ * only in a call. */
+int mi_kv_evict(void *const *layer_pools, void *kv_data, int64_t kv_layer_stride, float *scores,
+                int32_t num_layers, int64_t num_pages, int32_t page_size, int32_t num_kv_heads,
+                int32_t head_dim, int32_t dtype, const int32_t *kv_indptr,
+                const int32_t *kv_indices, const int32_t *kv_last_page_len, int32_t batch_size,
+                int32_t max_len, int32_t budget, int32_t recent, int32_t sinks, int32_t *kept,
+                int32_t *status, mi_stream_t stream);
 /* One decode (or prefill) step's page metadata, on the device.
  * Lane i is request slot lane_slots[i] (-1: padding lane) whose newest token
  * sits at lane_positions[i]. With grow != 0, a lane whose slot holds fewer

@@ -27,7 +27,7 @@ STAMP = LIB + ".sha256"
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
-    "-cudart", "static", "--expt-relaxed-constexpr",
+    "-cudart", "static", "--expt-relaxed-constexpr", "--threads", "8",
 ]
 
 

@@ -620,9 +620,8 @@ int launch_tc(DecodeParams p, void *ws, size_t ws_bytes, cudaStream_t s) {
   return check_launch("decode_tc_kernel");
 }
 
-// Shapes and alignments the workspace kernels (stream-K, then the ticket
-// kernel) serve; every other call runs the generic kernel, which needs no
-// workspace.
+}  // namespace
+
 bool decode_fast_shape(const void *q, int64_t qsb, int64_t qsh, const void *kv, const void *out,
                        int head_dim, int dtype, int group, int batch) {
   const bool half_type = dtype == MI_DTYPE_BF16 || dtype == MI_DTYPE_F16;
@@ -633,6 +632,8 @@ bool decode_fast_shape(const void *q, int64_t qsb, int64_t qsh, const void *kv, 
   return half_type && (head_dim == 64 || head_dim == 128) && group <= 16 && batch <= kMaxBatch &&
          aligned;
 }
+
+namespace {
 
 template <typename T>
 int launch_fast(const DecodeParams &p, void *ws, size_t ws_bytes, cudaStream_t s) {

@@ -97,6 +97,13 @@ struct SkParams {
   const void *rope_cos, *rope_sin;
   int rope_max;
   void *kv;  // the pool, for the new tokens' page writes
+  // Score form (mi_paged_decode_scores): the scaled logits (log2 units) of
+  // every token under every query head, [hq][logit_stride] with a request's
+  // tokens at (its first page position) * ps onward, and the rows'
+  // log2-sum-exp; decode_scores.cu turns them into weights afterwards.
+  float *logits, *lse2;
+  int64_t logit_stride;
+  const int32_t *rope_pos;  // optional RoPE position of each request's new token
 };
 
 constexpr int kSmemBatch = 1024;  // requests whose metadata fits the shared-memory copy
@@ -171,7 +178,7 @@ __device__ __forceinline__ void vsplit_run(const int32_t *ip, int B, int c4, int
   *hi = vsplit_page(ip, B, c4, x1, lane);
 }
 
-template <typename T, int D, bool G16, int HKV>
+template <typename T, int D, bool G16, int HKV, bool SCORES>
 __global__ void __launch_bounds__(kThreads, 1)
     decode_sk_kernel(const __grid_constant__ CUtensorMap tmap, const SkParams p) {
   constexpr int KS = D / 16, NT = D / 8, DH = D / 64;
@@ -256,7 +263,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                   (li % kLineRow) * 128);
     if (p.k_new == nullptr) return;
     const int pos = kvlen - 1;
-    if (pos < 0 || pos >= p.rope_max) return;
+    int rpos = pos;  // RoPE position: the slot, unless the cache lost tokens
+    if constexpr (SCORES)
+      if (p.rope_pos) rpos = p.rope_pos[b];
+    if (pos < 0 || rpos < 0 || rpos >= p.rope_max) return;
     const char *kb = static_cast<const char *>(p.k_new) + static_cast<int64_t>(b) * p.ksb * sizeof(T);
     const char *vb = static_cast<const char *>(p.v_new) + static_cast<int64_t>(b) * p.vsb * sizeof(T);
     for (int li = lane; li < 2 * HKV * kLineRow; li += 32) {
@@ -267,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (lane < 2 * kLineRow) {
       const char *tab = static_cast<const char *>(lane < kLineRow ? p.rope_cos : p.rope_sin);
-      prefetch_l1(tab + static_cast<int64_t>(pos) * D * sizeof(T) + (lane % kLineRow) * 128);
+      prefetch_l1(tab + static_cast<int64_t>(rpos) * D * sizeof(T) + (lane % kLineRow) * 128);
     } else if (lane == 2 * kLineRow) {
       prefetch_l1(p.indices + ip[b] + pos / p.ps);
     }
@@ -461,9 +471,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (p.k_new == nullptr) return;
     // fused append: the request's new token is its last, at kv_len - 1
     const int pos = kvlen - 1;
-    const bool rope_ok = pos >= 0 && pos < p.rope_max;
-    const T *cr = static_cast<const T *>(p.rope_cos) + static_cast<int64_t>(rope_ok ? pos : 0) * D;
-    const T *sr = static_cast<const T *>(p.rope_sin) + static_cast<int64_t>(rope_ok ? pos : 0) * D;
+    int rpos = pos;  // RoPE position: the slot, unless the cache lost tokens
+    if constexpr (SCORES)
+      if (p.rope_pos) rpos = p.rope_pos[b];
+    const bool rope_ok = pos >= 0 && rpos >= 0 && rpos < p.rope_max;
+    const T *cr = static_cast<const T *>(p.rope_cos) + static_cast<int64_t>(rope_ok ? rpos : 0) * D;
+    const T *sr = static_cast<const T *>(p.rope_sin) + static_cast<int64_t>(rope_ok ? rpos : 0) * D;
     // the position's cos and sin rows (D/4 chunks of 16 bytes), staged in
     // this warp's shared-memory slot below
     uint4 csv = make_uint4(0, 0, 0, 0);
@@ -657,6 +670,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float x1 = ok(tb) ? s0[1] * p.scale_log2 : -INFINITY;
       const float x2 = ok(tc) ? s1[0] * p.scale_log2 : -INFINITY;
       const float x3 = ok(td) ? s1[1] * p.scale_log2 : -INFINITY;
+      // score form: the tile's logits (-inf past the request and on bad pages)
+      int64_t lcol = 0;
+      bool lrow = false;
+      if constexpr (SCORES) {
+        lcol = static_cast<int64_t>(ip[rec.b] - base0) * p.ps + rec.tok0 + t * kTile;
+        lrow = lcol + kTile <= p.logit_stride;
+        if (gid < p.group && lrow) {
+          float *lg = p.logits + (h * p.group + gid) * p.logit_stride + lcol + 2 * tq;
+          *reinterpret_cast<float2 *>(lg) = make_float2(x0, x1);
+          *reinterpret_cast<float2 *>(lg + 8) = make_float2(x2, x3);
+        }
+      }
       float mx = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -677,6 +702,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float y1 = ok(tb) ? s0[3] * p.scale_log2 : -INFINITY;
         const float y2 = ok(tc) ? s1[2] * p.scale_log2 : -INFINITY;
         const float y3 = ok(td) ? s1[3] * p.scale_log2 : -INFINITY;
+        if constexpr (SCORES) {
+          if (gid + 8 < p.group && lrow) {
+            float *lg = p.logits + (h * p.group + gid + 8) * p.logit_stride + lcol + 2 * tq;
+            *reinterpret_cast<float2 *>(lg) = make_float2(y0, y1);
+            *reinterpret_cast<float2 *>(lg + 8) = make_float2(y2, y3);
+          }
+        }
         float my = fmaxf(fmaxf(y0, y1), fmaxf(y2, y3));
         my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, 1));
         my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, 2));
@@ -791,6 +823,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int i = 0; i < DPL; ++i) ob[i * 32 + lane] = Elt<T>::from(acc[i] * inv);
         if (p.lse && lane == 0)
           p.lse[b * p.hq + qrow] = L > 0.f ? (M + __log2f(L)) * kLn2 : -INFINITY;
+        if constexpr (SCORES) {
+          if (lane == 0) p.lse2[b * p.hq + qrow] = L > 0.f ? M + log2f(L) : -INFINITY;
+        }
       } else {
         float *po = p.part_o + (static_cast<int64_t>(slot) * p.hq + qrow) * D;
 #pragma unroll
@@ -892,6 +927,8 @@ __global__ void __launch_bounds__(64) decode_sk_merge_kernel(const SkParams p, i
   for (int i = 0; i < DPL; ++i) ob[i * 32 + lane] = Elt<T>::from(acc[i] * inv);
   if (p.lse && lane == 0)
     p.lse[b * p.hq + qrow] = wsum > 0.f ? (M + __log2f(wsum)) * kLn2 : -INFINITY;
+  if (p.lse2 && lane == 0)
+    p.lse2[b * p.hq + qrow] = wsum > 0.f ? M + log2f(wsum) : -INFINITY;
 }
 
 // ---------------------------------------------------------------------------
@@ -935,13 +972,14 @@ bool sk_layout(int hkv, int d, int group, int batch, SkLayout *L) {
   return false;
 }
 
-template <typename T, int D, bool G16, int HKV>
-int launch_sk_t(const SkArgs &a, const CUtensorMap &map, const SkParams &p, int grid,
+template <typename T, int D, bool G16, int HKV, bool SCORES>
+int launch_sk_k(const SkArgs &a, const CUtensorMap &map, const SkParams &p, int grid,
                 int smem) {
   static std::atomic<unsigned long long> attr_set{0};
-  if (smem_limit_once(attr_set, decode_sk_kernel<T, D, G16, HKV>, kSmemLimit) != cudaSuccess)
+  if (smem_limit_once(attr_set, decode_sk_kernel<T, D, G16, HKV, SCORES>, kSmemLimit) !=
+      cudaSuccess)
     return check_launch("decode_sk_kernel smem attribute");
-  cudaError_t e = launch_pdl(decode_sk_kernel<T, D, G16, HKV>, dim3(grid), dim3(kThreads), smem,
+  cudaError_t e = launch_pdl(decode_sk_kernel<T, D, G16, HKV, SCORES>, dim3(grid), dim3(kThreads), smem,
                              a.stream, map, p);
   if (e != cudaSuccess) return fail(MI_ERR_CUDA, "decode_sk_kernel launch: %s", cudaGetErrorString(e));
   const int warps = a.batch * a.hq;
@@ -950,6 +988,13 @@ int launch_sk_t(const SkArgs &a, const CUtensorMap &map, const SkParams &p, int 
   if (e != cudaSuccess)
     return fail(MI_ERR_CUDA, "decode_sk_merge_kernel launch: %s", cudaGetErrorString(e));
   return check_launch("decode_sk_merge_kernel");
+}
+
+template <typename T, int D, bool G16, int HKV>
+int launch_sk_t(const SkArgs &a, const CUtensorMap &map, const SkParams &p, int grid,
+                int smem) {
+  return a.logits ? launch_sk_k<T, D, G16, HKV, true>(a, map, p, grid, smem)
+                  : launch_sk_k<T, D, G16, HKV, false>(a, map, p, grid, smem);
 }
 
 template <typename T, int D, bool G16>
@@ -1050,6 +1095,10 @@ int launch_decode_sk(const SkArgs &a) {
     p.rope_max = a.rope_max;
     p.kv = const_cast<void *>(a.kv);
   }
+  p.logits = a.logits;
+  p.lse2 = a.lse2;
+  p.logit_stride = a.logit_stride;
+  p.rope_pos = a.rope_pos;
   const bool g16 = group > 8;
   if (a.dtype == MI_DTYPE_BF16) {
     if (a.d == 128)

@@ -26,8 +26,18 @@ struct SkArgs {
   int64_t ksb = 0, ksh = 0, vsb = 0, vsh = 0;
   const void *rope_cos = nullptr, *rope_sin = nullptr;
   int rope_max = 0;
+  // score form (mi_paged_decode_scores): scaled logits [hq][logit_stride] and
+  // log2-sum-exp [batch][hq] also come out; null: not wanted
+  float *logits = nullptr, *lse2 = nullptr;
+  int64_t logit_stride = 0;
+  const int32_t *rope_pos = nullptr;  // RoPE position per request (null: its last slot)
 };
 
+// Shapes and alignments the workspace kernels (stream-K, then the ticket
+// kernel) serve; every other call runs the generic kernel, which needs no
+// workspace.
+bool decode_fast_shape(const void *q, int64_t qsb, int64_t qsh, const void *kv, const void *out,
+                       int head_dim, int dtype, int group, int batch);
 // Workspace bytes the stream-K kernel needs for this shape.
 size_t decode_sk_workspace_bytes(int batch, int hq, int hkv, int d);
 // Launches the stream-K kernel; returns -1 (nothing launched) when the

@@ -171,12 +171,15 @@ __global__ void __launch_bounds__(kPoolThreads) slot_alloc_kernel(
   }
 }
 
-// Retire, part 1: zero every page of the listed slots in every layer.
-// grid: (n * maxp, layers); block (i*maxp + j, l) zeroes page j of slot i.
+// Retire or trim, part 1: zero the listed slots' pages from the keep-th on in
+// every layer (and their scores, where there are any).
+// grid: (n * (maxp - keep), layers); block (i*(maxp - keep) + j - keep, l)
+// zeroes page j of slot i.
 __global__ void __launch_bounds__(256) slot_zero_kernel(
     const int32_t *table, const int32_t *nump, int max_slots, int maxp, const int32_t *slots,
-    int n, int num_pages, void *const *layers, int64_t page_bytes) {
-  const int i = blockIdx.x / maxp, j = blockIdx.x % maxp;
+    int n, int num_pages, void *const *layers, int64_t page_bytes, int keep, float *scores,
+    int score_elems) {
+  const int i = blockIdx.x / (maxp - keep), j = keep + blockIdx.x % (maxp - keep);
   const int s = slots[i];
   if (s < 0 || s >= max_slots || j >= nump[s]) return;
   const int page = table[static_cast<int64_t>(s) * maxp + j];
@@ -186,13 +189,17 @@ __global__ void __launch_bounds__(256) slot_zero_kernel(
   const int64_t nvec = page_bytes / 16;
   const uint4 z = make_uint4(0, 0, 0, 0);
   for (int64_t k = threadIdx.x; k < nvec; k += blockDim.x) dst[k] = z;
+  if (scores) {
+    float *sc = scores + (static_cast<int64_t>(blockIdx.y) * num_pages + page) * score_elems;
+    for (int k = threadIdx.x; k < score_elems; k += blockDim.x) sc[k] = 0.f;
+  }
 }
 
-// Retire, part 2: append the slots' pages to the ring tail (slot order, then
-// allocation order) and empty the slots.
+// Retire or trim, part 2: append the slots' pages from the keep-th on to the
+// ring tail (slot order, then allocation order); the slots keep the others.
 __global__ void __launch_bounds__(kPoolThreads) slot_free_kernel(
     int32_t *ring, int32_t *ctrl, int num_pages, int32_t *table, int32_t *nump, int max_slots,
-    int maxp, const int32_t *slots, int n, int32_t *status) {
+    int maxp, const int32_t *slots, int n, int keep, int32_t *status) {
   __shared__ int s_warp[32];
   const int head = ctrl[0], free_count = ctrl[1];
   auto valid = [&](int s) { return s >= 0 && s < max_slots; };
@@ -200,7 +207,7 @@ __global__ void __launch_bounds__(kPoolThreads) slot_free_kernel(
   for (int base = 0; base < n; base += blockDim.x) {
     const int i = base + threadIdx.x;
     if (i < n && !valid(slots[i])) flag(status, MI_STATUS_BAD_BATCH_INDEX);
-    const int c = (i < n && valid(slots[i])) ? nump[slots[i]] : 0;
+    const int c = (i < n && valid(slots[i])) ? max(0, nump[slots[i]] - keep) : 0;
     int tot;
     block_excl_scan(c, s_warp, tot);
     carry += tot;
@@ -213,16 +220,17 @@ __global__ void __launch_bounds__(kPoolThreads) slot_free_kernel(
   for (int base = 0; base < n; base += blockDim.x) {
     const int i = base + threadIdx.x;
     const int s = (i < n && valid(slots[i])) ? slots[i] : -1;
-    const int c = s >= 0 ? nump[s] : 0;
+    const int c = s >= 0 ? max(0, nump[s] - keep) : 0;
     int tot;
     const int off = done + block_excl_scan(c, s_warp, tot);
     for (int j = 0; j < c; ++j)
-      ring[(head + free_count + off + j) % num_pages] = table[static_cast<int64_t>(s) * maxp + j];
+      ring[(head + free_count + off + j) % num_pages] =
+          table[static_cast<int64_t>(s) * maxp + keep + j];
     done += tot;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += blockDim.x)
-    if (valid(slots[i])) nump[slots[i]] = 0;
+    if (valid(slots[i])) nump[slots[i]] = min(nump[slots[i]], keep);
   if (threadIdx.x == 0) ctrl[1] = free_count + done;
 }
 
@@ -386,13 +394,45 @@ extern "C" int mi_slot_release(int32_t *free_ring, int32_t *pool_ctrl, int32_t n
     dim3 grid(static_cast<unsigned>(blocks), num_layers);
     mi::slot_zero_kernel<<<grid, 256, 0, s>>>(page_table, slot_num_pages, max_slots,
                                                 max_pages_per_slot, slots, n, num_pages,
-                                                layer_pools, page_bytes);
+                                                layer_pools, page_bytes, 0, nullptr, 0);
     int rc = mi::check_launch("slot_zero_kernel");
     if (rc) return rc;
   }
   mi::slot_free_kernel<<<1, mi::kPoolThreads, 0, s>>>(free_ring, pool_ctrl, num_pages,
                                                        page_table, slot_num_pages, max_slots,
-                                                       max_pages_per_slot, slots, n, status);
+                                                       max_pages_per_slot, slots, n, 0, status);
+  return mi::check_launch("slot_free_kernel");
+}
+
+extern "C" int mi_slot_trim(int32_t *free_ring, int32_t *pool_ctrl, int32_t num_pages,
+                            int32_t *page_table, int32_t *slot_num_pages, int32_t max_slots,
+                            int32_t max_pages_per_slot, const int32_t *slots, int32_t n,
+                            int32_t keep_pages, void *const *layer_pools, int32_t num_layers,
+                            int64_t page_bytes, float *scores, int32_t score_page_elems,
+                            int32_t *status, mi_stream_t stream) {
+  MI_REQUIRE(free_ring && pool_ctrl && page_table && slot_num_pages && num_pages >= 2 &&
+                 max_slots > 0 && max_pages_per_slot > 0 && n >= 0 && keep_pages >= 0,
+             "slot_trim: bad arguments");
+  if (n == 0 || keep_pages >= max_pages_per_slot) return MI_OK;
+  MI_REQUIRE(slots, "slot_trim: null slots");
+  MI_REQUIRE(!scores || score_page_elems > 0, "slot_trim: bad score_page_elems");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (num_layers > 0) {
+    MI_REQUIRE(layer_pools && page_bytes > 0 && page_bytes % 16 == 0,
+               "slot_trim: bad layer_pools/page_bytes");
+    const long long blocks = static_cast<long long>(n) * (max_pages_per_slot - keep_pages);
+    MI_REQUIRE(blocks < (1LL << 31) && num_layers <= 65535, "slot_trim: too many pages");
+    dim3 grid(static_cast<unsigned>(blocks), num_layers);
+    mi::slot_zero_kernel<<<grid, 256, 0, s>>>(page_table, slot_num_pages, max_slots,
+                                                max_pages_per_slot, slots, n, num_pages,
+                                                layer_pools, page_bytes, keep_pages, scores,
+                                                score_page_elems);
+    int rc = mi::check_launch("slot_zero_kernel");
+    if (rc) return rc;
+  }
+  mi::slot_free_kernel<<<1, mi::kPoolThreads, 0, s>>>(
+      free_ring, pool_ctrl, num_pages, page_table, slot_num_pages, max_slots, max_pages_per_slot,
+      slots, n, keep_pages, status);
   return mi::check_launch("slot_free_kernel");
 }
 

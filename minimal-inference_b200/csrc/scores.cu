@@ -1,0 +1,296 @@
+// Accumulated attention weights of cached tokens, per KV head:
+//   scores[page][h][slot] += sum over queries i and the group's heads g of
+//                            exp(q_ig . k_slot * sm_scale - lse_ig),
+// what an eviction by accumulated weight (evict.cu) ranks the cache by. The
+// reference keeps every token (its cache only grows); no counterpart there.
+//
+// Two forms:
+//   * Decode (one query per request): the stream-K decode kernel already has
+//     every logit, so its score form stores them (fp32, log2 units; 1/16 of
+//     the bytes of K and V at 4 heads per KV head, and L2 resident) and
+//     weights_kernel turns them into weights once the row sums are known:
+//     no second pass over K. Shapes outside that kernel run the generic form
+//     after the decode.
+//   * A prompt's last `window` queries, whose log-sum-exp the prefill
+//     attention returned (scores_tc.cu for 16-bit types; the generic kernel
+//     here for any type and head_dim).
+// Sums are fp32 and per token in a fixed order; the addition into `scores` is
+// one fp32 reduction per token and KV head (red.add), so a page listed once
+// gets the same bits every time, and one listed twice gets both sums.
+#include <algorithm>
+
+#include "decode_sk.cuh"
+#include "mi_common.cuh"
+#include "scores.cuh"
+
+namespace mi {
+namespace {
+
+__device__ __forceinline__ void red_add(float *p, float v) {
+  asm volatile("red.global.add.f32 [%0], %1;" ::"l"(p), "f"(v) : "memory");
+}
+
+// Request that holds page position `pos` (counted from indptr[0]).
+__device__ __forceinline__ int request_of(const int32_t *indptr, int batch, int pos) {
+  const int base = indptr[0];
+  int l = 0, h = batch - 1;
+  while (l < h) {
+    const int mid = (l + h + 1) >> 1;
+    if (indptr[mid] - base <= pos) l = mid; else h = mid - 1;
+  }
+  return l;
+}
+
+// ---- generic ---------------------------------------------------------------
+// Work item: 16 tokens of a page under one KV head. K rows in shared memory
+// as fp32 (row stride d + 1: the 16 tokens of a half-warp in different banks);
+// thread = (token, part): every 8th (query, group head) row, dot products in
+// fp32 over the whole head, the parts added in order at the end.
+constexpr int kGTok = 16, kGParts = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(kGTok *kGParts) scores_generic_kernel(const ScoreParams p) {
+  extern __shared__ float s_k[];  // [16][d + 1]
+  __shared__ float s_part[kGParts][kGTok];
+  const int total = p.indptr[p.batch] - p.indptr[0];
+  const int chunks = (p.ps + kGTok - 1) / kGTok;
+  const int64_t items = static_cast<int64_t>(total) * chunks * p.hkv;
+  const int tok = threadIdx.x % kGTok, part = threadIdx.x / kGTok;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const int h = static_cast<int>(it % p.hkv);
+    const int chunk = static_cast<int>(it / p.hkv % chunks);
+    const int pos = static_cast<int>(it / p.hkv / chunks);
+    const int b = request_of(p.indptr, p.batch, pos);
+    const int first = p.indptr[b] - p.indptr[0];
+    const int kvlen = kv_len_of(p.indptr, p.last, b, p.ps);
+    const int slot0 = chunk * kGTok;
+    const int j0 = (pos - first) * p.ps + slot0;  // the chunk's first token
+    const int nt = min(min(kGTok, p.ps - slot0), kvlen - j0);
+    if (nt <= 0) continue;
+    const int64_t page = p.indices[p.indptr[0] + pos];
+    if (page < 0 || page >= p.num_pages) {
+      if (threadIdx.x == 0) flag(p.status, MI_STATUS_BAD_PAGE);
+      continue;
+    }
+    // the request's queries: rows [q0, q0 + nq), the last `window` of them
+    int q0 = b, nq = 1;
+    if (p.qo_indptr) {
+      q0 = p.qo_indptr[b];
+      nq = p.qo_indptr[b + 1] - q0;
+      if (q0 < 0 || nq <= 0 || q0 + nq > p.total_q) {
+        if (nq != 0 && threadIdx.x == 0) flag(p.status, MI_STATUS_BAD_POSITION);
+        continue;
+      }
+    }
+    const int i0 = p.window > 0 ? max(0, nq - p.window) : 0;
+    __syncthreads();  // the previous item's readers are done
+    const T *kp = static_cast<const T *>(p.kv) +
+                  ((page * 2) * p.ps + slot0) * (static_cast<int64_t>(p.hkv) * p.d) +
+                  static_cast<int64_t>(h) * p.d;
+    for (int e = threadIdx.x; e < nt * p.d; e += blockDim.x) {
+      const int r = e / p.d, c = e % p.d;
+      s_k[r * (p.d + 1) + c] = Elt<T>::to(kp[static_cast<int64_t>(r) * p.hkv * p.d + c]);
+    }
+    __syncthreads();
+    float sum = 0.f;
+    if (tok < nt) {
+      const int j = j0 + tok;
+      const float *kr = s_k + tok * (p.d + 1);
+      // causal: query i sees tokens j <= kvlen - nq + i
+      const int lo = p.causal ? max(i0, j - (kvlen - nq)) : i0;
+      const int rows = max(0, nq - lo) * p.group;
+      for (int r = part; r < rows; r += kGParts) {
+        const int i = q0 + lo + r / p.group, hq = h * p.group + r % p.group;
+        const float l = p.lse[static_cast<int64_t>(i) * p.hq + hq];
+        if (l == -INFINITY) continue;  // a row that saw nothing
+        const T *qr = static_cast<const T *>(p.q) + i * p.qsn + hq * p.qsh;
+        float s = 0.f;
+        for (int c = 0; c < p.d; ++c) s = fmaf(Elt<T>::to(qr[c]), kr[c], s);
+        sum += expf(fmaf(s, p.scale, -l));
+      }
+    }
+    s_part[part][tok] = sum;
+    __syncthreads();
+    if (threadIdx.x < nt) {
+      float t = 0.f;
+      for (int i = 0; i < kGParts; ++i) t += s_part[i][threadIdx.x];
+      red_add(p.scores + (page * p.hkv + h) * p.ps + slot0 + threadIdx.x, t);
+    }
+  }
+}
+
+template <typename T>
+int launch_generic_t(const ScoreParams &p, cudaStream_t s) {
+  const int smem = kGTok * (p.d + 1) * 4;
+  scores_generic_kernel<T><<<num_sms() * 8, kGTok * kGParts, smem, s>>>(p);
+  return check_launch("scores_generic_kernel");
+}
+
+int launch_generic(const ScoreParams &p, int dtype, cudaStream_t s) {
+  switch (dtype) {
+    case MI_DTYPE_F32: return launch_generic_t<float>(p, s);
+    case MI_DTYPE_F16: return launch_generic_t<__half>(p, s);
+    default: return launch_generic_t<__nv_bfloat16>(p, s);
+  }
+}
+
+// ---- decode: stored logits to weights ----------------------------------------
+// One thread per (token, KV head): grid y = KV head, x strides over the page
+// positions' slots. Reads of a head's logits and the score additions are both
+// contiguous over the tokens of a page.
+__global__ void __launch_bounds__(256) weights_kernel(
+    const float *__restrict__ logits, int64_t stride, const float *__restrict__ lse2,
+    const int32_t *indptr, const int32_t *indices, const int32_t *last, int batch, int group,
+    int hq, int ps, int hkv, int64_t num_pages, float *scores) {
+  pdl_trigger();  // dependents wait for this grid themselves; it writes only scores
+  const int h = blockIdx.y;
+  const int base = indptr[0];
+  const int64_t n = min(static_cast<int64_t>(indptr[batch] - base) * ps, stride);
+  pdl_wait();
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const int pos = static_cast<int>(i / ps), slot = static_cast<int>(i % ps);
+    const int b = request_of(indptr, batch, pos);
+    const int first = indptr[b] - base;
+    if (static_cast<int64_t>(pos - first) * ps + slot >= kv_len_of(indptr, last, b, ps)) continue;
+    const int64_t page = indices[base + pos];
+    if (page < 0 || page >= num_pages) continue;  // (flagged by the decode)
+    const float *lg = logits + static_cast<int64_t>(h) * group * stride + i;
+    const float *l2 = lse2 + b * hq + h * group;
+    float w = 0.f;
+    for (int g = 0; g < group; ++g) w += exp2f(lg[g * stride] - l2[g]);
+    red_add(scores + (page * hkv + h) * ps + slot, w);
+  }
+}
+
+size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+
+}  // namespace
+}  // namespace mi
+
+extern "C" size_t mi_paged_decode_scores_scratch_size(int32_t batch_size, int32_t num_qo_heads,
+                                                      int32_t page_size, int64_t max_pages) {
+  if (batch_size <= 0 || num_qo_heads <= 0 || page_size <= 0 || max_pages <= 0) return 0;
+  return mi::up256(size_t(batch_size) * num_qo_heads * 4) +
+         size_t(max_pages) * page_size * num_qo_heads * 4;
+}
+
+extern "C" int mi_paged_decode_scores(
+    const void *q, int64_t q_stride_b, int64_t q_stride_h,
+    const void *k_new, int64_t k_stride_b, int64_t k_stride_h,
+    const void *v_new, int64_t v_stride_b, int64_t v_stride_h,
+    const void *rope_cos, const void *rope_sin, int32_t rope_max_pos,
+    const int32_t *rope_positions,
+    void *kv_data, int64_t num_pages, int32_t page_size, int32_t num_kv_heads,
+    int32_t head_dim, int32_t dtype,
+    const int32_t *kv_indptr, const int32_t *kv_indices, int64_t max_pages,
+    const int32_t *kv_last_page_len, int32_t batch_size, int32_t num_qo_heads, float sm_scale,
+    void *out, float *lse, float *scores, void *scratch, size_t scratch_bytes,
+    void *workspace, size_t workspace_bytes, int32_t *status, mi_stream_t stream) {
+  using namespace mi;
+  MI_REQUIRE(batch_size >= 0, "decode_scores: negative batch_size");
+  if (batch_size == 0) return MI_OK;
+  MI_REQUIRE(q && kv_data && kv_indptr && kv_indices && kv_last_page_len && out && scores &&
+                 scratch && workspace,
+             "decode_scores: null pointer argument");
+  MI_REQUIRE(page_size > 0 && num_kv_heads > 0 && head_dim > 0 && head_dim <= 256 &&
+                 num_pages > 0 && max_pages > 0,
+             "decode_scores: bad pool geometry");
+  MI_REQUIRE(num_qo_heads >= num_kv_heads && num_qo_heads % num_kv_heads == 0,
+             "decode_scores: num_qo_heads %d is not a multiple of num_kv_heads %d", num_qo_heads,
+             num_kv_heads);
+  MI_REQUIRE(dtype == MI_DTYPE_F32 || dtype == MI_DTYPE_F16 || dtype == MI_DTYPE_BF16,
+             "decode_scores: bad dtype %d", dtype);
+  MI_REQUIRE(!k_new || (v_new && rope_cos && rope_sin && rope_max_pos > 0),
+             "decode_scores: k_new needs v_new and the RoPE tables");
+  MI_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 256 == 0 &&
+                 reinterpret_cast<uintptr_t>(scratch) % 256 == 0,
+             "decode_scores: workspace and scratch must be 256-byte aligned");
+  const size_t need = mi_paged_decode_scores_scratch_size(batch_size, num_qo_heads, page_size,
+                                                          max_pages);
+  if (scratch_bytes < need)
+    return fail(MI_ERR_WORKSPACE, "decode_scores: scratch of %zu bytes, %zu needed",
+                scratch_bytes, need);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int group = num_qo_heads / num_kv_heads;
+  float *row_lse = static_cast<float *>(scratch);  // [batch][hq]
+  float *logits = reinterpret_cast<float *>(static_cast<unsigned char *>(scratch) +
+                                            up256(size_t(batch_size) * num_qo_heads * 4));
+  if (decode_fast_shape(q, q_stride_b, q_stride_h, kv_data, out, head_dim, dtype, group,
+                        batch_size)) {
+    SkArgs sk{q, q_stride_b, q_stride_h, kv_data, num_pages, page_size, num_kv_heads,
+              head_dim, dtype, kv_indptr, kv_indices, kv_last_page_len, batch_size,
+              num_qo_heads, sm_scale, out, lse, workspace, workspace_bytes, status, s};
+    if (k_new) {
+      sk.k_new = k_new;
+      sk.ksb = k_stride_b;
+      sk.ksh = k_stride_h;
+      sk.v_new = v_new;
+      sk.vsb = v_stride_b;
+      sk.vsh = v_stride_h;
+      sk.rope_cos = rope_cos;
+      sk.rope_sin = rope_sin;
+      sk.rope_max = rope_max_pos;
+      sk.rope_pos = rope_positions;
+    }
+    sk.logits = logits;
+    sk.lse2 = row_lse;
+    sk.logit_stride = max_pages * page_size;
+    const int rc = launch_decode_sk(sk);
+    if (rc > 0) return rc;
+    if (rc == 0) {
+      const int64_t blocks = (max_pages * page_size + 255) / 256;
+      const int x = static_cast<int>(std::min<int64_t>(blocks, 16 * num_sms() / num_kv_heads + 1));
+      const cudaError_t e = launch_pdl(weights_kernel, dim3(x, num_kv_heads), dim3(256), 0, s,
+                                       static_cast<const float *>(logits), sk.logit_stride,
+                                       static_cast<const float *>(row_lse), kv_indptr, kv_indices,
+                                       kv_last_page_len, batch_size, group, num_qo_heads,
+                                       page_size, num_kv_heads, num_pages, scores);
+      if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(MI_ERR_CUDA, "weights_kernel launch: %s", cudaGetErrorString(e));
+      }
+      return check_launch("weights_kernel");
+    }
+  }
+  if (k_new)
+    return fail(MI_ERR_UNSUPPORTED, "decode_scores: shape outside the fused append's coverage");
+  float *l = lse ? lse : row_lse;
+  const int rc = mi_paged_decode(q, q_stride_b, q_stride_h, kv_data, num_pages, page_size,
+                                 num_kv_heads, head_dim, dtype, kv_indptr, kv_indices,
+                                 kv_last_page_len, batch_size, num_qo_heads, sm_scale, out, l,
+                                 workspace, workspace_bytes, status, stream);
+  if (rc != MI_OK) return rc;
+  ScoreParams p{q, q_stride_b, q_stride_h, nullptr, batch_size, kv_data, num_pages, page_size,
+                num_kv_heads, head_dim, kv_indptr, kv_indices, kv_last_page_len, batch_size,
+                num_qo_heads, group, 0, 0, sm_scale, l, scores, status};
+  return launch_generic(p, dtype, s);
+}
+
+extern "C" int mi_paged_prefill_scores(
+    const void *q, int64_t q_stride_n, int64_t q_stride_h,
+    const int32_t *qo_indptr, int32_t total_q,
+    const void *kv_data, int64_t num_pages, int32_t page_size, int32_t num_kv_heads,
+    int32_t head_dim, int32_t dtype,
+    const int32_t *kv_indptr, const int32_t *kv_indices, const int32_t *kv_last_page_len,
+    int32_t batch_size, int32_t num_qo_heads, int32_t causal, int32_t window, float sm_scale,
+    const float *lse, float *scores, int32_t *status, mi_stream_t stream) {
+  using namespace mi;
+  MI_REQUIRE(total_q >= 0 && batch_size >= 0, "prefill_scores: negative total_q/batch_size");
+  if (total_q == 0 || batch_size == 0) return MI_OK;
+  MI_REQUIRE(q && qo_indptr && kv_data && kv_indptr && kv_indices && kv_last_page_len && lse &&
+                 scores,
+             "prefill_scores: null pointer argument");
+  MI_REQUIRE(page_size > 0 && num_kv_heads > 0 && head_dim > 0 && head_dim <= 256 &&
+                 num_pages > 0,
+             "prefill_scores: bad pool geometry");
+  MI_REQUIRE(num_qo_heads >= num_kv_heads && num_qo_heads % num_kv_heads == 0,
+             "prefill_scores: num_qo_heads %d is not a multiple of num_kv_heads %d",
+             num_qo_heads, num_kv_heads);
+  MI_REQUIRE(dtype == MI_DTYPE_F32 || dtype == MI_DTYPE_F16 || dtype == MI_DTYPE_BF16,
+             "prefill_scores: bad dtype %d", dtype);
+  ScoreParams p{q, q_stride_n, q_stride_h, qo_indptr, total_q, kv_data, num_pages, page_size,
+                num_kv_heads, head_dim, kv_indptr, kv_indices, kv_last_page_len, batch_size,
+                num_qo_heads, num_qo_heads / num_kv_heads, causal != 0, window, sm_scale, lse,
+                scores, status};
+  return launch_generic(p, dtype, reinterpret_cast<cudaStream_t>(stream));
+}

@@ -65,6 +65,18 @@ def need_on(name: str, t: torch.Tensor, device) -> torch.Tensor:
     return t
 
 
+def check_scores(scores: torch.Tensor, kv: torch.Tensor, device) -> torch.Tensor:
+    """Accumulated attention weights beside a ``[P, 2, ps, Hkv, D]`` pool:
+    contiguous fp32 ``[P, Hkv, ps]``."""
+    p, ps, hkv, _ = check_pool(kv)
+    if tuple(scores.shape) != (p, hkv, ps) or scores.dtype != torch.float32:
+        raise ValueError(f"scores must be float32 [{p}, {hkv}, {ps}], got "
+                         f"{scores.dtype} {tuple(scores.shape)}")
+    if not scores.is_contiguous():
+        raise ValueError("scores must be contiguous")
+    return need_on("scores", scores, device)
+
+
 def check_rows(name: str, t: torch.Tensor, min_rows: int, row_shape: tuple, dtype: torch.dtype,
                device) -> torch.Tensor:
     """A caller-provided output the kernels write as dense rows: ``[>= min_rows,

@@ -69,6 +69,20 @@ _SIGS = {
         _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
         _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_f,
         _c_p, _c_p, _c_p, _c_size, _c_p, _c_p], ctypes.c_int),
+    "mi_paged_decode_scores_scratch_size": ([_c_i32, _c_i32, _c_i32, _c_i64], _c_size),
+    "mi_paged_decode_scores": ([
+        _c_p, _c_i64, _c_i64,
+        _c_p, _c_i64, _c_i64,
+        _c_p, _c_i64, _c_i64,
+        _c_p, _c_p, _c_i32, _c_p,
+        _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
+        _c_p, _c_p, _c_i64, _c_p, _c_i32, _c_i32, _c_f,
+        _c_p, _c_p, _c_p, _c_p, _c_size, _c_p, _c_size, _c_p, _c_p], ctypes.c_int),
+    "mi_paged_prefill_scores": ([
+        _c_p, _c_i64, _c_i64, _c_p, _c_i32,
+        _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
+        _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_i32, _c_f,
+        _c_p, _c_p, _c_p, _c_p], ctypes.c_int),
     "mi_page_pool_init": ([_c_p, _c_p, _c_i32, _c_p], ctypes.c_int),
     "mi_page_alloc": ([_c_p, _c_p, _c_i32, _c_p, _c_i32, _c_p, _c_p, _c_p], ctypes.c_int),
     "mi_page_release": ([_c_p, _c_p, _c_i32, _c_p, _c_i32, _c_p, _c_i32, _c_i64, _c_p, _c_p],
@@ -77,6 +91,11 @@ _SIGS = {
                        _c_p], ctypes.c_int),
     "mi_slot_release": ([_c_p, _c_p, _c_i32, _c_p, _c_p, _c_i32, _c_i32, _c_p, _c_i32, _c_p,
                          _c_i32, _c_i64, _c_p, _c_p], ctypes.c_int),
+    "mi_slot_trim": ([_c_p, _c_p, _c_i32, _c_p, _c_p, _c_i32, _c_i32, _c_p, _c_i32, _c_i32, _c_p,
+                      _c_i32, _c_i64, _c_p, _c_i32, _c_p, _c_p], ctypes.c_int),
+    "mi_kv_evict": ([_c_p, _c_p, _c_i64, _c_p, _c_i32, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
+                     _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_i32, _c_i32, _c_p, _c_p, _c_p],
+                    ctypes.c_int),
     "mi_step_prepare": ([_c_p, _c_p, _c_i32, _c_p, _c_p, _c_i32, _c_i32, _c_p, _c_p, _c_i32,
                          _c_i32, _c_i32, _c_p, _c_p, _c_i32, _c_p, _c_p, _c_p, _c_p],
                         ctypes.c_int),
@@ -125,7 +144,11 @@ def header_symbols() -> list[str]:
 
 def call(name: str, *args) -> None:
     """Call entry point ``name``; raise MiError on a non-zero return."""
-    rc = getattr(lib(), name)(*args)
+    check(name, getattr(lib(), name)(*args))
+
+
+def check(name: str, rc: int) -> None:
+    """Raise MiError when entry point ``name`` returned non-zero."""
     if rc != 0:
         msg = lib().mi_last_error().decode(errors="replace")
         raise MiError(f"{name} failed (code {rc}): {msg}")

@@ -14,7 +14,8 @@ import math
 import torch
 
 from . import capi
-from ._tensor import check_pool, check_rows, dtype_code, need_i32, need_on, ptr, stream_of
+from ._tensor import (check_pool, check_rows, check_scores, dtype_code, need_i32, need_on,
+                      on_device_of, ptr, stream_of)
 
 
 class BatchDecodeWithPagedKVCacheWrapper:
@@ -58,8 +59,13 @@ class BatchDecodeWithPagedKVCacheWrapper:
                           scale=sm_scale if sm_scale is not None else 1.0 / math.sqrt(head_dim))
 
     def run(self, q: torch.Tensor, paged_kv_cache: torch.Tensor, out: torch.Tensor | None = None,
-            lse: torch.Tensor | None = None, return_lse: bool = False):
-        """``q [B, Hq, D]`` -> ``out [B, Hq, D]`` (and ``lse [B, Hq]``)."""
+            lse: torch.Tensor | None = None, return_lse: bool = False,
+            scores: torch.Tensor | None = None):
+        """``q [B, Hq, D]`` -> ``out [B, Hq, D]`` (and ``lse [B, Hq]``).
+
+        ``scores`` (extension): fp32 ``[P, Hkv, ps]``; the attention weight
+        each cached token receives, summed over its group's query heads, is
+        added to its entry (what ``page.evict_paged_kv_cache`` ranks by)."""
         pl = self._plan
         if pl is None:
             raise RuntimeError("plan() must be called before run()")
@@ -82,6 +88,12 @@ class BatchDecodeWithPagedKVCacheWrapper:
             check_rows("lse", lse, b, (pl["hq"],), torch.float32, dev)
         elif return_lse:
             lse = torch.empty((b, pl["hq"]), dtype=torch.float32, device=q.device)
+        if scores is not None:
+            check_scores(scores, paged_kv_cache, dev)
+            rc = self._run_scores(q, None, None, None, None, None, paged_kv_cache, out, lse,
+                                  scores, self.status)
+            capi.check("mi_paged_decode_scores", rc)
+            return (out, lse) if return_lse else out
         capi.call(
             "mi_paged_decode",
             q.data_ptr(), q.stride(0), q.stride(1),
@@ -92,13 +104,43 @@ class BatchDecodeWithPagedKVCacheWrapper:
             self.status.data_ptr(), stream_of(q))
         return (out, lse) if return_lse else out
 
+    def _run_scores(self, q, k, v, rope_cos, rope_sin, rope_positions, kv, out, lse, scores,
+                    status) -> int:
+        """``mi_paged_decode_scores`` on checked arguments; its return code.
+
+        The logits scratch comes from torch's allocator per call: calls on
+        different streams, and captured graphs, never share it."""
+        pl = self._plan
+        num_pages, ps, hkv, d = check_pool(kv)
+        b, pages = pl["batch"], pl["indices"].numel()
+        if b == 0 or pages == 0:
+            out[:b].zero_()  # requests without pages
+            if lse is not None:
+                lse[:b].fill_(-math.inf)
+            return 0
+        nbytes = capi.lib().mi_paged_decode_scores_scratch_size(b, pl["hq"], ps, pages)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
+        with on_device_of(kv):
+            return capi.lib().mi_paged_decode_scores(
+                q.data_ptr(), q.stride(0), q.stride(1),
+                ptr(k), k.stride(0) if k is not None else 0, k.stride(1) if k is not None else 0,
+                ptr(v), v.stride(0) if v is not None else 0, v.stride(1) if v is not None else 0,
+                ptr(rope_cos), ptr(rope_sin), rope_cos.shape[0] if rope_cos is not None else 0,
+                ptr(rope_positions), kv.data_ptr(), num_pages, ps, hkv, d, dtype_code(kv.dtype),
+                pl["indptr"].data_ptr(), pl["indices"].data_ptr(), pages,
+                pl["last"].data_ptr(), b, pl["hq"], pl["scale"], out.data_ptr(), ptr(lse),
+                scores.data_ptr(), scratch.data_ptr(), nbytes, self._ws.data_ptr(),
+                self._ws.numel() * self._ws.element_size(), status.data_ptr(), stream_of(q))
+
     def run_with_append(self, q: torch.Tensor, paged_kv_cache: torch.Tensor,
                         append_key: torch.Tensor, append_value: torch.Tensor,
                         rope_cos: torch.Tensor, rope_sin: torch.Tensor,
                         out: torch.Tensor | None = None,
                         status: torch.Tensor | None = None,
                         positions: torch.Tensor | None = None,
-                        scratch_page: int = -1) -> torch.Tensor:
+                        scratch_page: int = -1,
+                        scores: torch.Tensor | None = None,
+                        rope_positions: torch.Tensor | None = None) -> torch.Tensor:
         """A decode step with its append fused in (extension, no FlashInfer
         counterpart): ``q`` are the raw queries ``[B, Hq, D]``,
         ``append_key``/``append_value`` the raw new K / V ``[B, Hkv, D]`` of
@@ -110,7 +152,12 @@ class BatchDecodeWithPagedKVCacheWrapper:
         ``scratch_page`` passed to the append when given (a scheduler's
         padded lanes have no pages and append into its scratch page; the
         fused kernel leaves such lanes out). Device-side problems are
-        flagged in ``status`` (default: this wrapper's)."""
+        flagged in ``status`` (default: this wrapper's).
+
+        ``scores``: as in ``run``. ``rope_positions`` (int32 ``[B]``, with
+        ``scores`` only): the new tokens' RoPE positions where the cache has
+        lost tokens to eviction and a token's slot is no longer its
+        position."""
         pl = self._plan
         if pl is None:
             raise RuntimeError("plan() must be called before run_with_append()")
@@ -137,17 +184,29 @@ class BatchDecodeWithPagedKVCacheWrapper:
         else:
             check_rows("out", out, b, (pl["hq"], d), dt, dev)
         st = self.status if status is None else need_i32("status", status, dev)
-        lib = capi.lib()
-        rc = lib.mi_paged_decode_append(
-            q.data_ptr(), q.stride(0), q.stride(1),
-            append_key.data_ptr(), append_key.stride(0), append_key.stride(1),
-            append_value.data_ptr(), append_value.stride(0), append_value.stride(1),
-            rope_cos.data_ptr(), rope_sin.data_ptr(), rope_cos.shape[0],
-            paged_kv_cache.data_ptr(), num_pages, ps, hkv, d, dtype_code(dt),
-            pl["indptr"].data_ptr(), pl["indices"].data_ptr(), pl["last"].data_ptr(), b,
-            pl["hq"], pl["scale"], out.data_ptr(), None,
-            self._ws.data_ptr(), self._ws.numel() * self._ws.element_size(), st.data_ptr(),
-            stream_of(q))
+        if scores is not None:
+            check_scores(scores, paged_kv_cache, dev)
+            if rope_positions is not None:
+                need_i32("rope_positions", rope_positions, dev)
+                if rope_positions.shape != (b,):
+                    raise ValueError(f"rope_positions must be [{b}]")
+            rc = self._run_scores(q, append_key, append_value, rope_cos, rope_sin,
+                                  rope_positions, paged_kv_cache, out, None, scores, st)
+            name = "mi_paged_decode_scores"
+        elif rope_positions is not None:
+            raise ValueError("rope_positions goes with scores")
+        else:
+            name = "mi_paged_decode_append"
+            rc = capi.lib().mi_paged_decode_append(
+                q.data_ptr(), q.stride(0), q.stride(1),
+                append_key.data_ptr(), append_key.stride(0), append_key.stride(1),
+                append_value.data_ptr(), append_value.stride(0), append_value.stride(1),
+                rope_cos.data_ptr(), rope_sin.data_ptr(), rope_cos.shape[0],
+                paged_kv_cache.data_ptr(), num_pages, ps, hkv, d, dtype_code(dt),
+                pl["indptr"].data_ptr(), pl["indices"].data_ptr(), pl["last"].data_ptr(), b,
+                pl["hq"], pl["scale"], out.data_ptr(), None,
+                self._ws.data_ptr(), self._ws.numel() * self._ws.element_size(), st.data_ptr(),
+                stream_of(q))
         if rc == capi.ERR_UNSUPPORTED:
             from .page import append_paged_kv_cache
             if positions is None:
@@ -159,11 +218,10 @@ class BatchDecodeWithPagedKVCacheWrapper:
                                   torch.arange(b, dtype=torch.int32, device=dev), positions,
                                   paged_kv_cache, pl["indices"], pl["indptr"], pl["last"],
                                   rope_cos=rope_cos, rope_sin=rope_sin, q=q[:b], q_out=q_rot,
+                                  rope_positions=rope_positions,
                                   scratch_page=scratch_page, status=st)
-            return self.run(q_rot, paged_kv_cache, out=out)
-        if rc != 0:
-            msg = lib.mi_last_error().decode(errors="replace")
-            raise capi.MiError(f"mi_paged_decode_append failed (code {rc}): {msg}")
+            return self.run(q_rot, paged_kv_cache, out=out, scores=scores)
+        capi.check(name, rc)
         return out
 
     def check_status(self) -> None:

@@ -11,7 +11,8 @@ from __future__ import annotations
 import torch
 
 from . import capi
-from ._tensor import check_pool, dtype_code, need_i32, need_on, ptr, stream_of
+from ._tensor import (check_pool, check_scores, dtype_code, need_i32, need_on, on_device_of, ptr,
+                      stream_of)
 
 
 def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor,
@@ -88,3 +89,67 @@ def append_paged_kv_cache(append_key: torch.Tensor, append_value: torch.Tensor,
         ptr(q_out), q_out.stride(0) if q is not None else 0,
         q_out.stride(1) if q is not None else 0, hq,
         scratch_page, ptr(status), stream_of(paged_kv_cache))
+
+
+def evict_paged_kv_cache(paged_kv_cache: torch.Tensor, scores: torch.Tensor,
+                         kv_indices: torch.Tensor, kv_indptr: torch.Tensor,
+                         kv_last_page_len: torch.Tensor, budget: int, *, recent: int = 0,
+                         sinks: int = 0, max_len: int | None = None, return_kept: bool = False,
+                         status: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Cut every request with more than ``budget`` cached tokens to ``budget``,
+    in place, by accumulated attention weight (``mi_kv_evict``).
+
+    ``paged_kv_cache`` is one layer's pool ``[P, 2, ps, Hkv, D]`` with
+    ``scores [P, Hkv, ps]``, or the layers' pools in one tensor ``[L, P, 2,
+    ps, Hkv, D]`` with ``scores [L, P, Hkv, ps]``; layers and KV heads choose
+    by themselves. Kept are the first ``sinks`` slots, the last ``recent`` ones
+    and the best-scored between them (equal scores: the lowest slot).
+    Afterwards the kept tokens fill slots ``0 .. budget - 1``, the recent ones
+    last and in order, the others in no particular order; scores move along and
+    are 0 behind. The page table tensors are not changed.
+
+    ``max_len``: an upper bound of the requests' lengths (default: all of
+    ``kv_indices``' slots; at most 819200). Returns, with ``return_kept``, int32
+    ``[(L,) B, Hkv, budget]``: the slot each kept token came from (-1: none)."""
+    stacked = paged_kv_cache.dim() == 6
+    layers = paged_kv_cache.shape[0] if stacked else 1
+    if stacked and not paged_kv_cache.is_contiguous():
+        raise ValueError("paged kv cache must be contiguous")
+    if stacked and layers == 0:
+        raise ValueError("no layers")
+    kv = paged_kv_cache[0] if stacked else paged_kv_cache
+    num_pages, ps, hkv, d = check_pool(kv)
+    dev = paged_kv_cache.device
+    if stacked:
+        if scores.dim() != 4 or scores.shape[0] != layers or not scores.is_contiguous():
+            raise ValueError(f"scores must be a contiguous [{layers}, {num_pages}, {hkv}, {ps}]")
+        check_scores(scores[0], kv, dev)
+    else:
+        check_scores(scores, kv, dev)
+    for name, t in (("kv_indices", kv_indices), ("kv_indptr", kv_indptr),
+                    ("kv_last_page_len", kv_last_page_len)):
+        need_i32(name, t, dev)
+    batch = kv_indptr.numel() - 1
+    if batch < 0 or kv_last_page_len.numel() < batch:
+        raise ValueError("kv_indptr needs batch + 1 entries and kv_last_page_len batch")
+    if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
+        raise ValueError(f"need 0 <= recent + sinks <= budget, got {recent} + {sinks}, {budget}")
+    if max_len is None:
+        max_len = max(1, kv_indices.numel() * ps)
+    if max_len < 1:
+        raise ValueError(f"max_len must be positive, got {max_len}")
+    if status is not None:
+        need_i32("status", status, dev)
+    stream = stream_of(paged_kv_cache)
+    kept = None
+    if return_kept:
+        shape = (batch, hkv, budget)
+        kept = torch.empty((layers, *shape) if stacked else shape, dtype=torch.int32, device=dev)
+    with on_device_of(paged_kv_cache):
+        capi.call("mi_kv_evict", None, paged_kv_cache.data_ptr(),
+                  paged_kv_cache.stride(0) if stacked else 0, scores.data_ptr(), layers,
+                  num_pages, ps, hkv, d, dtype_code(paged_kv_cache.dtype), kv_indptr.data_ptr(),
+                  kv_indices.data_ptr(), kv_last_page_len.data_ptr(), batch,
+                  min(max_len, 2 ** 31 - 1), budget, recent, sinks, ptr(kept), ptr(status),
+                  stream)
+    return kept

@@ -12,7 +12,8 @@ import math
 import torch
 
 from . import capi
-from ._tensor import check_pool, check_rows, dtype_code, need_i32, need_on, ptr, stream_of
+from ._tensor import (check_pool, check_rows, check_scores, dtype_code, need_i32, need_on,
+                      on_device_of, ptr, stream_of)
 
 
 class BatchPrefillWithPagedKVCacheWrapper:
@@ -95,6 +96,42 @@ class BatchPrefillWithPagedKVCacheWrapper:
             pl["batch"], pl["hq"], int(pl["causal"]), pl["scale"], out.data_ptr(), ptr(lse),
             self._ws.data_ptr(), ws_bytes, self.status.data_ptr(), stream_of(q))
         return (out, lse) if return_lse else out
+
+    def accumulate_scores(self, q: torch.Tensor, paged_kv_cache: torch.Tensor,
+                          lse: torch.Tensor, scores: torch.Tensor, window: int = 0) -> None:
+        """Add to ``scores [P, Hkv, ps]`` (fp32) the attention weight each
+        cached token received from the last ``window`` queries of its request
+        (0: from all of them), summed over the group's query heads.
+
+        ``q`` and ``lse [total_q, Hq]`` are those of this plan's ``run(q,
+        paged_kv_cache, return_lse=True)``. No FlashInfer counterpart: the
+        scores rank tokens for ``page.evict_paged_kv_cache``."""
+        pl = self._plan
+        if pl is None:
+            raise RuntimeError("plan() must be called before accumulate_scores()")
+        num_pages, ps, hkv, d = check_pool(paged_kv_cache)
+        if (ps, hkv, d) != (pl["ps"], pl["hkv"], pl["d"]):
+            raise ValueError("paged kv cache geometry differs from plan()")
+        if q.dim() != 3 or q.shape[1] != pl["hq"] or q.shape[2] != d:
+            raise ValueError(f"q must be [total_q, {pl['hq']}, {d}], got {tuple(q.shape)}")
+        if q.stride(-1) != 1 or q.dtype != paged_kv_cache.dtype:
+            raise ValueError("q needs the pool dtype and a unit stride on head_dim")
+        if window < 0:
+            raise ValueError(f"window must be >= 0, got {window}")
+        dev = self._ws.device
+        need_on("q", q, dev)
+        need_on("paged_kv_cache", paged_kv_cache, dev)
+        total_q = q.shape[0]
+        check_rows("lse", lse, total_q, (pl["hq"],), torch.float32, dev)
+        check_scores(scores, paged_kv_cache, dev)
+        with on_device_of(q):
+            capi.call(
+                "mi_paged_prefill_scores",
+                q.data_ptr(), q.stride(0), q.stride(1), pl["qo"].data_ptr(), total_q,
+                paged_kv_cache.data_ptr(), num_pages, ps, hkv, d, dtype_code(q.dtype),
+                pl["indptr"].data_ptr(), pl["indices"].data_ptr(), pl["last"].data_ptr(),
+                pl["batch"], pl["hq"], int(pl["causal"]), min(window, 2 ** 31 - 1), pl["scale"],
+                lse.data_ptr(), scores.data_ptr(), self.status.data_ptr(), stream_of(q))
 
     def check_status(self) -> None:
         w = int(self.status.item())
