@@ -254,8 +254,9 @@ int mi_paged_prefill(
  * mi_paged_prefill_scores: the weights given by the last `window` queries of
  * each request (window <= 0: all of them) of an mi_paged_prefill call with
  * the same arguments, from the lse it returned ([total_q][num_qo_heads],
- * natural log; -inf: the row saw nothing). Queries are not read outside the
- * window.
+ * natural log; -inf: the row saw nothing). The result does not depend on
+ * queries outside the window. workspace: that of mi_paged_prefill (the same
+ * rules; NULL: fixed round robin).
  * ------------------------------------------------------------------------- */
 size_t mi_paged_decode_scores_scratch_size(int32_t batch_size, int32_t num_qo_heads,
                                            int32_t page_size, int64_t max_pages);
@@ -278,7 +279,8 @@ int mi_paged_prefill_scores(
     int32_t head_dim, int32_t dtype,
     const int32_t *kv_indptr, const int32_t *kv_indices, const int32_t *kv_last_page_len,
     int32_t batch_size, int32_t num_qo_heads, int32_t causal, int32_t window, float sm_scale,
-    const float *lse, float *scores, int32_t *status, mi_stream_t stream);
+    const float *lse, float *scores, void *workspace, size_t workspace_bytes, int32_t *status,
+    mi_stream_t stream);
 
 /* ---------------------------------------------------------------------------
  * (4) Device page pool (replaces PagedKVCache's free list, scheduler.py:168-221)

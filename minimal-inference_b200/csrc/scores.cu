@@ -273,7 +273,8 @@ extern "C" int mi_paged_prefill_scores(
     int32_t head_dim, int32_t dtype,
     const int32_t *kv_indptr, const int32_t *kv_indices, const int32_t *kv_last_page_len,
     int32_t batch_size, int32_t num_qo_heads, int32_t causal, int32_t window, float sm_scale,
-    const float *lse, float *scores, int32_t *status, mi_stream_t stream) {
+    const float *lse, float *scores, void *workspace, size_t workspace_bytes, int32_t *status,
+    mi_stream_t stream) {
   using namespace mi;
   MI_REQUIRE(total_q >= 0 && batch_size >= 0, "prefill_scores: negative total_q/batch_size");
   if (total_q == 0 || batch_size == 0) return MI_OK;
@@ -292,5 +293,12 @@ extern "C" int mi_paged_prefill_scores(
                 num_kv_heads, head_dim, kv_indptr, kv_indices, kv_last_page_len, batch_size,
                 num_qo_heads, num_qo_heads / num_kv_heads, causal != 0, window, sm_scale, lse,
                 scores, status};
-  return launch_generic(p, dtype, reinterpret_cast<cudaStream_t>(stream));
+  // words 2 and 3 of the prefill workspace (0 and 1 are the prefill's own)
+  unsigned *ctr = nullptr;
+  if (workspace && workspace_bytes >= 256 && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0)
+    ctr = static_cast<unsigned *>(workspace) + 2;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int rc = launch_scores_tc(p, dtype, ctr, s);
+  if (rc >= 0) return rc;
+  return launch_generic(p, dtype, s);
 }

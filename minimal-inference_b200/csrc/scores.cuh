@@ -22,4 +22,9 @@ struct ScoreParams {
   int32_t *status;
 };
 
+// Tensor-core prompt scores (scores_tc.cu). ctr: two work-item counters, zero
+// between calls, or null (fixed round robin). Returns -1 (nothing launched)
+// when the shape or layout is outside its coverage.
+int launch_scores_tc(const ScoreParams &p, int dtype, unsigned *ctr, cudaStream_t s);
+
 }  // namespace mi

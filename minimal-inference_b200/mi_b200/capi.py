@@ -82,7 +82,7 @@ _SIGS = {
         _c_p, _c_i64, _c_i64, _c_p, _c_i32,
         _c_p, _c_i64, _c_i32, _c_i32, _c_i32, _c_i32,
         _c_p, _c_p, _c_p, _c_i32, _c_i32, _c_i32, _c_i32, _c_f,
-        _c_p, _c_p, _c_p, _c_p], ctypes.c_int),
+        _c_p, _c_p, _c_p, _c_size, _c_p, _c_p], ctypes.c_int),
     "mi_page_pool_init": ([_c_p, _c_p, _c_i32, _c_p], ctypes.c_int),
     "mi_page_alloc": ([_c_p, _c_p, _c_i32, _c_p, _c_i32, _c_p, _c_p, _c_p], ctypes.c_int),
     "mi_page_release": ([_c_p, _c_p, _c_i32, _c_p, _c_i32, _c_p, _c_i32, _c_i64, _c_p, _c_p],

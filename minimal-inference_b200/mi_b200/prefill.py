@@ -131,7 +131,9 @@ class BatchPrefillWithPagedKVCacheWrapper:
                 paged_kv_cache.data_ptr(), num_pages, ps, hkv, d, dtype_code(q.dtype),
                 pl["indptr"].data_ptr(), pl["indices"].data_ptr(), pl["last"].data_ptr(),
                 pl["batch"], pl["hq"], int(pl["causal"]), min(window, 2 ** 31 - 1), pl["scale"],
-                lse.data_ptr(), scores.data_ptr(), self.status.data_ptr(), stream_of(q))
+                lse.data_ptr(), scores.data_ptr(), self._ws.data_ptr(),
+                self._ws.numel() * self._ws.element_size(), self.status.data_ptr(),
+                stream_of(q))
 
     def check_status(self) -> None:
         w = int(self.status.item())
