@@ -18,6 +18,11 @@ Two ways to use it:
   ``step_prepare`` (page growth + CSR for a step) and ``slot_release``
   (retire) never synchronise.
 
+``track_scores`` adds one fp32 score per cached token, KV head and layer
+(``score_data``), which the attention calls accumulate and ``evict`` ranks by:
+a slot longer than a budget is cut to it and its freed pages return to the
+pool. Scores of free pages are zero, as their K and V are.
+
 The host keeps an exact mirror of the free-page count (``num_free_pages``),
 so admission control and the out-of-pages error (scheduler.py:208-214) need
 no device read.
@@ -29,7 +34,7 @@ import math
 import torch
 
 from . import capi
-from ._tensor import stream_of
+from ._tensor import dtype_code, need_i32, ptr, stream_of
 
 
 class _FreeCount:
@@ -45,7 +50,7 @@ class _FreeCount:
 class PagedKVCache:
     def __init__(self, config, max_batch_size: int, max_seq_len: int, page_size: int,
                  device, dtype: torch.dtype, num_layers: int | None = None,
-                 num_kv_heads: int | None = None):
+                 num_kv_heads: int | None = None, track_scores: bool = False):
         device = torch.device(device)
         if device.type != "cuda":
             raise capi.MiError("PagedKVCache lives on a CUDA device (no CPU fallback)")
@@ -75,6 +80,9 @@ class PagedKVCache:
         self.status = torch.zeros(1, **i32)
         capi.call("mi_page_pool_init", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
                   self.max_num_pages, stream_of(self.free_ring))
+        # accumulated attention weights [layers, P, Hkv, ps], or None
+        self.score_data = (torch.zeros(self.num_layers, self.max_num_pages, self.num_kv_heads,
+                                       page_size, device=device) if track_scores else None)
         self.num_free_pages = self.max_num_pages - 1
         self.free_pages = _FreeCount(self)
 
@@ -100,6 +108,9 @@ class PagedKVCache:
         if not pages:
             return
         t = torch.tensor(pages, dtype=torch.int32, device=self.device)
+        if self.score_data is not None:
+            own = [p for p in pages if 0 <= p < self.max_num_pages]  # others are flagged below
+            self.score_data.index_fill_(1, torch.tensor(own, device=self.device), 0.0)
         capi.call("mi_page_release", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
                   self.max_num_pages, t.data_ptr(), len(pages), self.layer_ptrs.data_ptr(),
                   self.num_layers, self.page_bytes, self.status.data_ptr(), stream_of(t))
@@ -119,12 +130,58 @@ class PagedKVCache:
 
     def slot_release(self, slots: torch.Tensor, total_pages: int) -> None:
         """Retire: zero every page of ``slots`` in every layer and free them."""
+        if self.score_data is not None:
+            self._trim(slots, 0, total_pages)
+            return
         capi.call("mi_slot_release", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
                   self.max_num_pages, self.page_table.data_ptr(), self.slot_num_pages.data_ptr(),
                   self.max_batch_size, self.max_pages_per_seq, slots.data_ptr(), slots.numel(),
                   self.layer_ptrs.data_ptr(), self.num_layers, self.page_bytes,
                   self.status.data_ptr(), stream_of(slots))
         self.num_free_pages += total_pages
+
+    def _trim(self, slots: torch.Tensor, keep_pages: int, freed_pages: int) -> None:
+        """Free the pages of ``slots`` from the ``keep_pages``-th on, zeroed."""
+        sc = self.score_data
+        capi.call("mi_slot_trim", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
+                  self.max_num_pages, self.page_table.data_ptr(), self.slot_num_pages.data_ptr(),
+                  self.max_batch_size, self.max_pages_per_seq, slots.data_ptr(), slots.numel(),
+                  keep_pages, self.layer_ptrs.data_ptr(), self.num_layers, self.page_bytes,
+                  ptr(sc), self.num_kv_heads * self.page_size, self.status.data_ptr(),
+                  stream_of(slots))
+        self.num_free_pages += freed_pages
+
+    def evict(self, slots: torch.Tensor, lengths: torch.Tensor, budget: int,
+              freed_pages: int, *, recent: int = 0, sinks: int = 0) -> None:
+        """Cut each of ``slots`` (holding ``lengths`` tokens, both device int32)
+        to at most ``budget`` tokens by accumulated score, in every layer and KV
+        head (``page.evict_paged_kv_cache``), and free the pages past the
+        budget. ``freed_pages``: how many that is over all slots (the caller
+        knows the lengths). A slot's next token goes to position ``min(length,
+        budget)`` of its pages. Does not synchronise."""
+        if self.score_data is None:
+            raise RuntimeError("evict() needs PagedKVCache(track_scores=True)")
+        if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
+            raise ValueError(f"need 0 <= recent + sinks <= budget, got {recent} + {sinks}, "
+                             f"{budget}")
+        n = slots.numel()
+        need_i32("slots", slots, self.page_table.device)
+        need_i32("lengths", lengths, self.page_table.device)
+        if lengths.numel() != n:
+            raise ValueError("slots and lengths differ in length")
+        if n == 0:
+            return
+        i32 = dict(dtype=torch.int32, device=self.device)
+        indptr, last, unused = (torch.empty(n + 1, **i32), torch.empty(n, **i32),
+                                torch.empty(n, **i32))
+        indices = torch.empty(n * self.max_pages_per_seq, **i32)
+        self.step_prepare(slots, lengths - 1, indptr, indices, last, unused, grow=False)
+        capi.call("mi_kv_evict", self.layer_ptrs.data_ptr(), None, 0, self.score_data.data_ptr(),
+                  self.num_layers, self.max_num_pages, self.page_size, self.num_kv_heads,
+                  self.head_dim, dtype_code(self.dtype), indptr.data_ptr(), indices.data_ptr(),
+                  last.data_ptr(), n, self.max_pages_per_seq * self.page_size, budget, recent,
+                  sinks, None, self.status.data_ptr(), stream_of(slots))
+        self._trim(slots, math.ceil(budget / self.page_size), freed_pages)
 
     def step_prepare(self, lane_slots: torch.Tensor, lane_positions: torch.Tensor,
                      kv_indptr: torch.Tensor, kv_indices: torch.Tensor,

@@ -192,7 +192,8 @@ class Attention(nn.Module):
             out = be.wrapper.run_with_append(
                 q, kv_data, k, v, be.rope_cos, be.rope_sin,
                 out=be.out_buffer(n, hq, d, x.dtype), status=be.status,
-                positions=be.positions, scratch_page=be.paged_kv_cache.scratch_page)
+                positions=be.positions, scratch_page=be.paged_kv_cache.scratch_page,
+                scores=be.layer_scores(layer), rope_positions=be.rope_positions)
         else:
             q_rot = be.q_buffer(n, hq, d, x.dtype)
             # RoPE on Q and K + K/V scatter into the pages: one launch
@@ -201,7 +202,14 @@ class Attention(nn.Module):
                                   be.kv_page_indices, be.kv_page_indptr, be.kv_last_page_len,
                                   rope_cos=be.rope_cos, rope_sin=be.rope_sin, q=q, q_out=q_rot,
                                   scratch_page=be.paged_kv_cache.scratch_page, status=be.status)
-            out = be.wrapper.run(q_rot, kv_data, out=be.out_buffer(n, hq, d, x.dtype))
+            out = be.out_buffer(n, hq, d, x.dtype)
+            scores = be.layer_scores(layer)
+            if scores is None:
+                be.wrapper.run(q_rot, kv_data, out=out)
+            else:  # the prompt's last queries rank its tokens for eviction
+                _, lse = be.wrapper.run(q_rot, kv_data, out=out, return_lse=True)
+                be.wrapper.accumulate_scores(q_rot, kv_data, lse, scores,
+                                             window=be.score_window)
         if proj_out is not None:
             torch.mm(out.view(n, hq * d), self._o_wt, out=proj_out)
             return proj_out.view(bsz, seq_len, -1)

@@ -21,6 +21,12 @@ What differs is where the work runs:
 * decode graphs are captured per batch bucket {1,2,4,8,16,32,48,64}
   (:350); padding lanes carry slot -1, so their append lands on the scratch
   page and their attention is empty.
+
+Two additions to the contract: a request may ask for top-k, top-p and min-p
+sampling, a seed and log-probabilities (``sampling.sample_tokens``), and
+``kv_budget`` bounds the tokens each request keeps in the cache: attention
+accumulates each cached token's weight, and a request that outgrows the budget
+by a page is cut back to it (``PagedKVCache.evict``).
 """
 from __future__ import annotations
 
@@ -28,6 +34,7 @@ import asyncio
 import enum
 import logging
 import math
+import random
 import threading
 import time
 from collections import deque
@@ -39,6 +46,7 @@ import torch.nn.functional as F
 from .decode import BatchDecodeWithPagedKVCacheWrapper
 from .kv_cache import PagedKVCache
 from .prefill import BatchPrefillWithPagedKVCacheWrapper
+from .sampling import sample_tokens
 
 logger = logging.getLogger(__name__)
 
@@ -69,6 +77,26 @@ class Request:
     last_token_time: float = 0.0
     token_queue: asyncio.Queue = field(default_factory=asyncio.Queue)
     loop: asyncio.AbstractEventLoop | None = None
+    # sampling beyond temperature (sampling.sample_tokens)
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    seed: int | None = None       # the request's own random numbers
+    logprobs: bool = False        # fill token_logprobs
+    token_logprobs: list[float] = field(default_factory=list)
+    cached_len: int = 0           # tokens in the cache: current_position less the evicted
+    _rng: random.Random | None = field(default=None, repr=False)
+
+    @property
+    def plain_sampling(self) -> bool:
+        """Whether temperature alone describes the request's sampling."""
+        return (self.top_k <= 0 and self.top_p >= 1 and self.min_p <= 0 and self.seed is None
+                and not self.logprobs)
+
+    def next_uniform(self) -> float:
+        if self._rng is None:
+            self._rng = random.Random(self.seed)
+        return self._rng.randrange(1 << 24) / (1 << 24)  # exact in fp32, below 1
 
 
 class AttentionBackend:
@@ -81,7 +109,7 @@ class AttentionBackend:
 
     def __init__(self, paged_kv_cache, wrapper, mode, kv_page_indptr, kv_page_indices,
                  kv_last_page_len, append_indptr, batch_indices, positions, status=None,
-                 q_buf=None, out_buf=None):
+                 q_buf=None, out_buf=None, rope_positions=None, score_window=0):
         self.paged_kv_cache = paged_kv_cache
         self.wrapper = wrapper
         self.mode = mode
@@ -93,6 +121,9 @@ class AttentionBackend:
         self.positions = positions
         self.status = status if status is not None else paged_kv_cache.status
         self.rope_cos = self.rope_sin = None
+        # decode with eviction: the tokens' RoPE positions (positions are slots)
+        self.rope_positions = rope_positions
+        self.score_window = score_window
         self._q_buf, self._out_buf = q_buf, out_buf
         self._layer_idx = 0
 
@@ -100,6 +131,11 @@ class AttentionBackend:
         idx = self._layer_idx
         self._layer_idx += 1
         return idx
+
+    def layer_scores(self, layer: int):
+        """The layer's accumulated attention weights, or None (not tracked)."""
+        sc = getattr(self.paged_kv_cache, "score_data", None)
+        return None if sc is None else sc[layer]
 
     def q_buffer(self, n, hq, d, dtype):
         if self._q_buf is None or self._q_buf.shape[0] < n:
@@ -155,15 +191,18 @@ class CUDAGraphRunner:
     The graph holds the whole step: page growth + CSR (``mi_step_prepare``),
     the model forward with fused append and paged decode per layer, and the
     logits. Inputs are one int32 tensor ``[3, bs]`` (slot, position, last
-    token per lane; slot -1 = padding), copied in before each replay.
+    token per lane; slot -1 = padding), copied in before each replay; a cache
+    that evicts has a fourth row, the RoPE positions, and the position row
+    counts the tokens in the cache.
     """
 
     def __init__(self, batch_size, kv_cache: PagedKVCache, num_heads, head_dim, dtype, device):
         self.batch_size = bs = batch_size
         i32 = dict(dtype=torch.int32, device=device)
-        self.inputs = torch.zeros(3, bs, **i32)
+        nrows = 3 if kv_cache.score_data is None else 4
+        self.inputs = torch.zeros(nrows, bs, **i32)
         self.inputs[0].fill_(-1)
-        self.host_inputs = torch.zeros(3, bs, dtype=torch.int32).pin_memory()
+        self.host_inputs = torch.zeros(nrows, bs, dtype=torch.int32).pin_memory()
         self.kv_page_indptr = torch.zeros(bs + 1, **i32)
         self.kv_page_indices = torch.zeros(bs * kv_cache.max_pages_per_seq, **i32)
         self.kv_last_page_len = torch.ones(bs, **i32)
@@ -189,7 +228,9 @@ class CUDAGraphRunner:
                                    self.kv_page_indices, self.kv_last_page_len,
                                    self.append_indptr, self.batch_indices,
                                    self.append_positions, q_buf=self.q_buf,
-                                   out_buf=self.out_buf)
+                                   out_buf=self.out_buf,
+                                   rope_positions=(self.inputs[3] if self.inputs.shape[0] > 3
+                                                   else None))
         decode_wrapper.plan(self.kv_page_indptr, self.kv_page_indices, self.kv_last_page_len,
                             model.layers[0].self_attn.num_heads,
                             model.layers[0].self_attn.num_kv_heads, config.head_dim, page_size,
@@ -206,7 +247,7 @@ class CUDAGraphRunner:
             self.logits = self._step(model, backend)
         self._backend = backend
 
-    def replay(self, slots, positions, tokens) -> torch.Tensor:
+    def replay(self, slots, positions, tokens, rope_positions=None) -> torch.Tensor:
         n = len(slots)
         h = self.host_inputs
         h[0].fill_(-1)
@@ -215,6 +256,9 @@ class CUDAGraphRunner:
         h[0, :n] = torch.tensor(slots, dtype=torch.int32)
         h[1, :n] = torch.tensor(positions, dtype=torch.int32)
         h[2, :n] = torch.tensor(tokens, dtype=torch.int32)
+        if h.shape[0] > 3:
+            h[3].zero_()
+            h[3, :n] = torch.tensor(rope_positions, dtype=torch.int32)
         self.inputs.copy_(h, non_blocking=True)
         self.graph.replay()
         return self.logits
@@ -226,7 +270,13 @@ class Scheduler:
                  eos_token_ids: set[int] | None = None, use_flashinfer: bool = True,
                  use_cuda_graph: bool = True, teacher_tokens: dict | None = None,
                  num_kv_heads: int | None = None, num_heads: int | None = None,
-                 max_prefill_tokens: int = 32768):
+                 max_prefill_tokens: int = 32768, kv_budget: int | None = None,
+                 kv_recent: int | None = None, kv_sinks: int = 4, kv_score_window: int = 64):
+        """``kv_budget`` (extension): tokens a request keeps in the cache, per
+        layer and KV head; the last ``kv_recent`` (default a quarter of it) and
+        the first ``kv_sinks`` always stay, the others by the attention weight
+        they received from the prompt's last ``kv_score_window`` queries
+        (0: all) and from every decode step. None: nothing is evicted."""
         global EOS_TOKEN_IDS
         if eos_token_ids is not None:
             EOS_TOKEN_IDS = eos_token_ids
@@ -247,8 +297,18 @@ class Scheduler:
         self.num_heads = num_heads or attn0.num_heads
         self.num_kv_heads = num_kv_heads or attn0.num_kv_heads
         self.max_prefill_tokens = max_prefill_tokens
+        self.kv_budget = kv_budget
+        if kv_budget is not None:
+            self.kv_sinks = kv_sinks
+            self.kv_recent = kv_budget // 4 if kv_recent is None else kv_recent
+            self.kv_score_window = kv_score_window
+            if (kv_budget < 1 or kv_sinks < 0 or self.kv_recent < 0 or kv_score_window < 0
+                    or kv_sinks + self.kv_recent > kv_budget):
+                raise ValueError("kv_budget needs 0 <= kv_recent + kv_sinks <= kv_budget and "
+                                 "kv_score_window >= 0")
         self.kv_cache = PagedKVCache(config, max_batch_size, max_seq_len, page_size, device, dtype,
-                                     num_kv_heads=self.num_kv_heads)
+                                     num_kv_heads=self.num_kv_heads,
+                                     track_scores=kv_budget is not None)
         ws = 256 * 1024 * 1024
         self._prefill_workspace = torch.empty(ws, dtype=torch.uint8, device=device)
         self._decode_workspace = torch.zeros(ws, dtype=torch.uint8, device=device)
@@ -380,24 +440,72 @@ class Scheduler:
                                    self.num_kv_heads, self.config.head_dim, self.page_size,
                                    causal=True, q_data_type=self.dtype)
         backend = AttentionBackend(self.kv_cache, self._prefill_wrapper, "prefill", indptr,
-                                   indices, last, qo_t, batch_indices, positions)
+                                   indices, last, qo_t, batch_indices, positions,
+                                   score_window=self.kv_score_window if self.kv_budget else 0)
         last_rows = qo_t[1:].long() - 1                  # each request's last token
         rows = self.model(ids.unsqueeze(0), position_ids=None, attn_backend=backend,
                           logits_rows=last_rows)[0]
         if self.record_logits:
             self.step_logits.append(("prefill", [r.request_id for r in reqs], rows.float().cpu()))
-        next_tokens = sample_rows(rows, [r.temperature for r in reqs]).tolist()
+        next_tokens = self._sample(rows, reqs)
         now = time.perf_counter()
         for req, n, tok in zip(reqs, lens, next_tokens):
             tok = self._forced(req, tok)
-            req.generated_tokens.append(tok)
-            req.current_position = n
-            req.status = RequestStatus.DECODING
+            req.current_position = req.cached_len = n
             req.prefill_done_time = req.last_token_time = now
+            if tok < 0:
+                self._fail(req)
+                continue
+            req.generated_tokens.append(tok)
+            req.status = RequestStatus.DECODING
             self._push_token(req, tok)
             if tok in EOS_TOKEN_IDS or len(req.generated_tokens) >= req.max_new_tokens:
                 req.status = RequestStatus.FINISHED
                 req.finish_reason = "stop" if tok in EOS_TOKEN_IDS else "length"
+        if self.kv_budget is not None:
+            self._evict([r for r in reqs if r.status == RequestStatus.DECODING
+                         and r.cached_len > self.kv_budget])
+
+    def _sample(self, rows: torch.Tensor, reqs: list) -> list[int]:
+        """Next tokens of ``rows [B, V]``; temperature alone goes through
+        ``sample_rows`` as the reference's does, anything more through
+        ``sample_tokens``. -1: a row without a logit above -inf."""
+        if all(r.plain_sampling for r in reqs):
+            return sample_rows(rows, [r.temperature for r in reqs]).tolist()
+        shared = torch.rand(len(reqs))  # torch's generator, as sample_rows uses
+        floats = torch.tensor([
+            [float(u) if r.seed is None else r.next_uniform() for r, u in zip(reqs, shared)],
+            [r.temperature for r in reqs], [r.top_p for r in reqs], [r.min_p for r in reqs]],
+            dtype=torch.float32).to(self.device)
+        top_k = torch.tensor([min(max(r.top_k, 0), rows.shape[1]) for r in reqs],
+                             dtype=torch.int32, device=self.device)
+        tokens, logprobs = sample_tokens(rows, floats[0], floats[1], top_k, floats[2], floats[3],
+                                         return_logprobs=True)
+        if any(r.logprobs for r in reqs):
+            for r, lp in zip(reqs, logprobs.tolist()):
+                if r.logprobs:
+                    r.token_logprobs.append(lp)
+        return tokens.tolist()
+
+    @staticmethod
+    def _fail(req) -> None:
+        """No token could be chosen (every logit NaN or -inf): the request ends."""
+        req.status = RequestStatus.FINISHED
+        req.finish_reason = "error"
+
+    @torch.inference_mode()
+    def _evict(self, reqs: list) -> None:
+        """Cut the cached tokens of ``reqs`` (each past the budget) to it."""
+        if not reqs:
+            return
+        i32 = dict(dtype=torch.int32, device=self.device)
+        pages = lambda n: math.ceil(n / self.page_size)  # noqa: E731
+        freed = sum(pages(r.cached_len) - pages(self.kv_budget) for r in reqs)
+        self.kv_cache.evict(torch.tensor([r.batch_slot for r in reqs], **i32),
+                            torch.tensor([r.cached_len for r in reqs], **i32), self.kv_budget,
+                            freed, recent=self.kv_recent, sinks=self.kv_sinks)
+        for r in reqs:
+            r.cached_len = self.kv_budget
 
     def _forced(self, req, tok: int) -> int:
         if self.teacher_tokens and req.request_id in self.teacher_tokens:
@@ -416,38 +524,47 @@ class Scheduler:
         b = len(decoding)
         # pages this step grows (host mirror of the device allocator)
         grow = sum(1 for r in decoding
-                   if math.ceil((r.current_position + 1) / self.page_size)
-                   > math.ceil(r.current_position / self.page_size))
+                   if math.ceil((r.cached_len + 1) / self.page_size)
+                   > math.ceil(r.cached_len / self.page_size))
         if grow > self.kv_cache.num_free_pages:
             raise RuntimeError(
                 f"Cannot allocate {grow} pages, only {self.kv_cache.num_free_pages} free")
         self.kv_cache.num_free_pages -= grow
         slots = [r.batch_slot for r in decoding]
-        positions = [r.current_position for r in decoding]
+        positions = [r.cached_len for r in decoding]
+        rope = [r.current_position for r in decoding] if self.kv_budget is not None else None
         tokens = [r.generated_tokens[-1] for r in decoding]
         bucket = next((bs for bs in GRAPH_BATCH_SIZES if bs >= b), 0)
         runner = self._graph_runners.get(bucket) if bucket else None
         if runner is not None:
-            logits = runner.replay(slots, positions, tokens)[:b]
+            logits = runner.replay(slots, positions, tokens, rope)[:b]
         else:
-            logits = self._decode_eager(slots, positions, tokens)
+            logits = self._decode_eager(slots, positions, tokens, rope)
         if self.record_logits:
             self.step_logits.append(("decode", [r.request_id for r in decoding],
                                      logits.float().cpu()))
-        next_tokens = sample_rows(logits, [r.temperature for r in decoding]).tolist()
+        next_tokens = self._sample(logits, decoding)
         now = time.perf_counter()
         for req, tok in zip(decoding, next_tokens):
             tok = self._forced(req, tok)
-            req.generated_tokens.append(tok)
             req.current_position += 1
+            req.cached_len += 1
             req.last_token_time = now
+            if tok < 0:
+                self._fail(req)
+                continue
+            req.generated_tokens.append(tok)
             self._push_token(req, tok)
             if (tok in EOS_TOKEN_IDS or len(req.generated_tokens) >= req.max_new_tokens
                     or req.current_position >= self.max_seq_len):
                 req.status = RequestStatus.FINISHED
                 req.finish_reason = "stop" if tok in EOS_TOKEN_IDS else "length"
 
-    def _decode_eager(self, slots, positions, tokens) -> torch.Tensor:
+        if self.kv_budget is not None:
+            self._evict([r for r in decoding if r.status == RequestStatus.DECODING
+                         and r.cached_len >= self.kv_budget + self.page_size])
+
+    def _decode_eager(self, slots, positions, tokens, rope=None) -> torch.Tensor:
         dev = self.device
         b = len(slots)
         i32 = dict(dtype=torch.int32, device=dev)
@@ -461,7 +578,9 @@ class Scheduler:
         self._decode_wrapper.plan(indptr, indices, last, self.num_heads, self.num_kv_heads,
                                   self.config.head_dim, self.page_size, q_data_type=self.dtype)
         backend = AttentionBackend(self.kv_cache, self._decode_wrapper, "decode", indptr, indices,
-                                   last, torch.arange(b + 1, **i32), torch.arange(b, **i32), apos)
+                                   last, torch.arange(b + 1, **i32), torch.arange(b, **i32), apos,
+                                   rope_positions=(torch.tensor(rope, **i32)
+                                                   if rope is not None else None))
         ids = torch.tensor(tokens, dtype=torch.long, device=dev).unsqueeze(1)
         return self.model(ids, position_ids=None, attn_backend=backend)[:, -1, :]
 
@@ -480,9 +599,9 @@ class Scheduler:
             else:
                 still.append(req)
         if done:
-            # pages held = ceil(current_position / ps): the last sampled token was
-            # never appended
-            held = sum(math.ceil(r.current_position / self.page_size) for r in done)
+            # pages held = ceil(cached_len / ps) (cached_len is current_position
+            # unless tokens were evicted): the last sampled token was never appended
+            held = sum(math.ceil(r.cached_len / self.page_size) for r in done)
             slots = torch.tensor([r.batch_slot for r in done], dtype=torch.int32,
                                  device=self.device)
             self.kv_cache.slot_release(slots, held)
