@@ -16,23 +16,38 @@
 // near-flat row of 150,000 tokens still has 2^-44 of resolution per token.
 //
 // One thread-block cluster per row (1 to 8 CTAs); each CTA keeps its slice of
-// the row in shared memory as ordered keys, read from HBM once. The passes
-// exchange through distributed shared memory:
-//   1. the largest composite (which is the greedy answer);
-//   2. a 256-bin histogram of counts and masses over -log2 w in steps of 1/8
-//      (linear in x: bins of the key's own bits would hold most of a row in a
-//      few bins): the bin where the filter's prefix ends;
+// the row in shared memory, read from HBM once. The passes exchange through
+// distributed shared memory:
+//   1. the largest logit (packed maxima while the slice comes in);
+//   2. a histogram over -log2 w in steps of 1/16, from which follows a bin at
+//      or above which everything that may be kept lies: token counts for
+//      top-k; for top-p counts times each bin's least or most weight, against
+//      p times the row's mass. Only the tokens within 2^-16 of the largest
+//      weight are counted at first (most of a row's are not, and an atomic a
+//      token would be the kernel's largest cost); where that does not decide,
+//      a second pass counts down to 2^-64 (nothing below 2^-45 can be drawn).
+//      The mass is summed in the same pass, with the exact 64-bit exponential
+//      within 2^-8, and below it with the hardware's exp2, whose 2^-22 of so
+//      little is as good;
 //   3. if no more than kCap tokens lie at or above that bin (the usual case),
-//      they are gathered, sorted in registers, and every filter and the draw
-//      happen on that list; else the range of composites the threshold lies in
-//      is divided by 256 until kCap tokens are left in it, and the draw is one
-//      more pass over the row: mass per warp, then the warp that holds u's
-//      place scans its tokens.
+//      they are gathered, one per thread, and every filter and the draw happen
+//      on that list with exact weights: a thread finds its token's rank and the
+//      mass before it by comparing with all others (tens of tokens as a rule;
+//      sorting needs more barriers than that takes);
+//   4. else ("wide" sets) the histogram brackets the bin where the prefix ends
+//      (exactly for counts; for masses between the bins' least and most
+//      weights), and divisions of the bracket's range of composites by 256,
+//      with exact masses, narrow the threshold down until kCap tokens are left
+//      in it. The draw is then one more pass over the row: mass per warp, then
+//      the warp that holds u's place scans its tokens.
+// The histogram's bins are linear in x: bins of the key's own bits would hold
+// most of a row in a few bins.
 #include <cooperative_groups.h>
 
 #include <algorithm>
 
 #include "mi_common.cuh"
+#include "umma.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -42,11 +57,15 @@ namespace {
 constexpr int kSThreads = 512;
 constexpr int kSWarps = kSThreads / 32;
 constexpr int kBins = 256;
-constexpr int kCap = 512;        // tokens resolved by sorting (one per thread)
+constexpr int kCap = 512;        // tokens resolved on a list (one per thread)
 constexpr int kMaxCluster = 8;   // portable cluster size
 constexpr int kIdxBits = 18;     // vocabulary <= 2^18
 constexpr uint32_t kIdxMask = (1u << kIdxBits) - 1;
 constexpr int kWeightBits = 44;  // the largest weight is 2^44
+constexpr int kFine = 1024;      // bins of 1/16 of -log2 w (two per thread)
+constexpr int kNear = 256;       // the bins of the first pass: down to 2^-16
+constexpr float kExact = 128.f;  // exact weights down to 2^-8
+constexpr float kRound = 8388608.f;  // adding it rounds to an integer, in the low bits
 constexpr int kLimb = 15;        // histogram masses: three 15-bit limbs in 32-bit counters
 constexpr int kMaxSlice = (1 << 17) - 1;  // limb sums: 2^17 tokens * 2^15 stay below 2^32
 
@@ -72,6 +91,18 @@ template <typename T> struct KeyOf;
 template <> struct KeyOf<__nv_bfloat16> {
   using K = uint16_t;
   static constexpr uint32_t kNone = 0x007F;
+  static constexpr K kEmpty = 0xFF80;  // -inf
+  __device__ static K bits(float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); }
+  __device__ static float raw(K b) { return __uint_as_float(static_cast<uint32_t>(b) << 16); }
+  // larger of each pair of numbers in a word (a NaN loses)
+  __device__ static uint32_t max_word(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162 *>(&a),
+                                     *reinterpret_cast<__nv_bfloat162 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&m);
+  }
+  __device__ static float max_of(uint32_t w) {
+    return fmaxf(raw(static_cast<K>(w)), raw(static_cast<K>(w >> 16)));
+  }
   __device__ static K key(uint16_t b) {
     if ((b & 0x7FFF) > 0x7F80) return 0;
     if (b == 0x8000) b = 0;
@@ -85,6 +116,17 @@ template <> struct KeyOf<__nv_bfloat16> {
 template <> struct KeyOf<__half> {
   using K = uint16_t;
   static constexpr uint32_t kNone = 0x03FF;
+  static constexpr K kEmpty = 0xFC00;
+  __device__ static K bits(float x) { return __half_as_ushort(__float2half_rn(x)); }
+  __device__ static float raw(K b) { return __half2float(__ushort_as_half(b)); }
+  __device__ static uint32_t max_word(uint32_t a, uint32_t b) {
+    const __half2 m =
+        __hmax2(*reinterpret_cast<__half2 *>(&a), *reinterpret_cast<__half2 *>(&b));
+    return *reinterpret_cast<const uint32_t *>(&m);
+  }
+  __device__ static float max_of(uint32_t w) {
+    return fmaxf(raw(static_cast<K>(w)), raw(static_cast<K>(w >> 16)));
+  }
   __device__ static K key(uint16_t b) {
     if ((b & 0x7FFF) > 0x7C00) return 0;
     if (b == 0x8000) b = 0;
@@ -98,6 +140,13 @@ template <> struct KeyOf<__half> {
 template <> struct KeyOf<float> {
   using K = uint32_t;
   static constexpr uint32_t kNone = 0x007FFFFF;
+  static constexpr K kEmpty = 0xFF800000u;
+  __device__ static K bits(float x) { return __float_as_uint(x); }
+  __device__ static float raw(K b) { return __uint_as_float(b); }
+  __device__ static uint32_t max_word(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
+  __device__ static float max_of(uint32_t w) { return __uint_as_float(w); }
   __device__ static K key(uint32_t b) {
     if ((b & 0x7FFFFFFFu) > 0x7F800000u) return 0;
     if (b == 0x80000000u) b = 0;
@@ -117,25 +166,48 @@ __device__ __forceinline__ uint32_t comp_idx(u64 c) {
   return kIdxMask - (static_cast<uint32_t>(c) & kIdxMask);
 }
 
-// A row's weights: functions of the key alone, the same in every pass.
+// A row's weights: functions of the logit alone, the same in every pass.
 struct RowW {
-  double xmax, inv_t;
-  float fmax, fscale;  // bins: 8 log2(e) / T
+  double xmax, c;       // c: log2(e) / T
+  float fmax_, fscale;  // fine bins: 16 log2(e) / T
+  const double *table;  // 2^(j / 32), shared memory
 
-  __device__ double weight_f(float x) const {
-    if (x == fmax) return 1.0;  // (also +inf among +inf)
-    const double d = static_cast<double>(x) - xmax;
-    return d == -INFINITY ? 0.0 : exp(d * inv_t);
+  // exp((x - xmax) / T) * 2^44 as a 64-bit float, from 2^t = 2^n 2^(j/32) 2^r:
+  // |r| <= 1/64, and the series of 2^r to r^4 leaves 2^-39. No branches, so
+  // the chains of a vector's tokens overlap.
+  __device__ double scaled(float x) const {
+    const double t = fmax((static_cast<double>(x) - xmax) * c, -64.0);  // (NaN: -64)
+    constexpr double kMagic = 6755399441055744.0 / 32;  // 1.5 * 2^52 in steps of 1/32
+    const double kd = t + kMagic;
+    const int k = __double2loint(kd);  // round(32 t)
+    const double r = t - (kd - kMagic);
+    double q = 0.009618129107628477;  // ln2^n / n!
+    q = fma(q, r, 0.05550410866482158);
+    q = fma(q, r, 0.2402265069591007);
+    q = fma(q, r, 0.6931471805599453);
+    const double m = table[k & 31];
+    double w = fma(q * r, m, m);
+    w = __hiloint2double(__double2hiint(w) + (((k >> 5) + kWeightBits) << 20),
+                         __double2loint(w));
+    return t > -64.0 ? w : 0.0;
   }
-  __device__ u64 weight(float x) const {
-    return __double2ull_rn(weight_f(x) * static_cast<double>(1ull << kWeightBits));
+  static __device__ u64 whole(double w) {  // nearest integer, by adding 2^52 (w <= 2^44)
+    return static_cast<u64>(__double_as_longlong(w + 4503599627370496.0)) & ((1ull << 52) - 1);
   }
-  // monotone in x: each of the subtraction, product and truncation is
-  __device__ int bin(float x) const {
-    if (x == fmax) return 0;
-    const float t = (fmax - x) * fscale;
-    return t >= kBins - 1 ? kBins - 1 : static_cast<int>(t);
-  }
+  __device__ u64 weight(float x) const { return whole(scaled(x)); }
+  // -log2 w in sixteenths (monotone in x: each of the subtraction and product
+  // is); +inf or NaN for -inf and NaN logits, which no comparison takes in
+  __device__ float steps(float x) const { return (fmax_ - x) * fscale; }
+  // whether its bin, the nearest integer, is at most b
+  __device__ bool within(float x, int b) const { return steps(x) + kRound <= kRound + b; }
+};
+
+// A place in the order, as a logit and a token: x is kept by a threshold when
+// it is larger, or as large with no larger index.
+struct Place {
+  float x;
+  uint32_t i;
+  __device__ bool takes(float y, uint32_t j) const { return y > x || (y == x && j <= i); }
 };
 
 struct __align__(16) Bin {
@@ -143,15 +215,24 @@ struct __align__(16) Bin {
 };
 
 struct Shared {
+  double table[32];
+  uint32_t fine[2][kFine];  // one buffer per search
   Bin hist[2][kBins];
   u64 list[kCap];   // this CTA's gathered composites
-  u64 sorted[kCap];
+  ulonglong2 pairs[kCap];           // the gathered list: composite, weight
+  float2 queue[kSWarps][64];        // per warp: tokens waiting for their weight
+  u64 acc[4];                       // integer sums over the list
   u64 scan[kSWarps];
+  uint32_t warp_n[kSWarps];
+  float warp_hi[kSWarps];
   u64 wsum[kSWarps];
+  double dsum[kSWarps], dsum2[kSWarps];
   // read by the other CTAs of the cluster, each written once before a barrier
-  u64 maxc;
-  double lsum;
-  u64 mass;
+  float maxv;
+  double lsum;       // sum of exp(x - max), temperature 1
+  double total[2];   // mass, per search
+  u64 mass, over;
+  uint32_t first;    // lowest token with the largest logit
   uint32_t list_n[2];
   // block-wide results
   u64 r_u64[4];
@@ -163,50 +244,28 @@ __device__ __forceinline__ u64 shfl_up64(u64 v, int o) {
   return __shfl_up_sync(0xffffffffu, v, o);
 }
 
-// Inclusive block scan of one 64-bit integer per thread.
-__device__ u64 block_scan(u64 v, u64 *s) {
+// Inclusive block scan of one 64-bit value per thread (in a fixed order).
+template <typename V>
+__device__ V block_scan(V v, void *buf) {
+  V *s = static_cast<V *>(buf);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const u64 y = shfl_up64(v, o);
+    const V y = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += y;
   }
   __syncthreads();  // (s may still be read from an earlier call)
   if (lane == 31) s[warp] = v;
   __syncthreads();
-  u64 before = 0;
+  V before = 0;
 #pragma unroll
   for (int i = 0; i < kSWarps; ++i)
     if (i < warp) before += s[i];
   return v + before;
 }
 
-// Sorts one 64-bit value per thread, descending over threadIdx.
-__device__ u64 block_sort_desc(u64 v, u64 *buf) {
-  const int t = threadIdx.x;
-#pragma unroll 1
-  for (int k = 2; k <= kSThreads; k <<= 1) {
-#pragma unroll 1
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      u64 o;
-      if (j >= 32) {
-        __syncthreads();
-        buf[t] = v;
-        __syncthreads();
-        o = buf[t ^ j];
-      } else {
-        o = __shfl_xor_sync(0xffffffffu, v, j);
-      }
-      const bool keep_max = ((t & j) == 0) == ((t & k) == 0);
-      v = keep_max ? (v > o ? v : o) : (v < o ? v : o);
-    }
-  }
-  __syncthreads();
-  return v;
-}
-
 template <typename T>
-__global__ void __launch_bounds__(kSThreads) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams p) {
   using KO = KeyOf<T>;
   using K = typename KO::K;
   constexpr int VEC = 16 / sizeof(K);
@@ -229,51 +288,72 @@ __global__ void __launch_bounds__(kSThreads) sample_kernel(const SampleParams p)
   const int per_warp = (nvec + kSWarps - 1) / kSWarps;  // a warp's vectors are consecutive
   const int v0 = min(nvec, warp * per_warp), v1 = min(nvec, v0 + per_warp);
 
-  for (int i = tid; i < 2 * kBins; i += kSThreads) sh.hist[0][i] = Bin{0, 0, 0, 0};
+  for (int i = tid; i < 2 * kFine; i += kSThreads) sh.fine[0][i] = 0;
   if (tid < 2) sh.list_n[tid] = 0;
-  if (tid == 0) sh.token = -1;
+  if (tid < 4) sh.acc[tid] = 0;
+  if (tid < 32) sh.table[tid] = exp2(tid * (1.0 / 32));
+  if (tid == 0) {
+    sh.token = -1;
+    sh.first = 0xFFFFFFFFu;
+  }
 
-  // ---- 1. the slice into shared memory; its largest composite --------------
-  u64 best = 0;
-  for (int v = v0 + lane; v < v1; v += 32) {
-    const int i0 = v * VEC - pad;  // first token of the vector
-    K k[VEC];
-    if (i0 >= 0 && i0 + VEC <= n) {
-      const uint4 raw = *reinterpret_cast<const uint4 *>(src + i0);
-      const K *e = reinterpret_cast<const K *>(&raw);
+  // ---- 1. the slice into shared memory; its largest logit ---------------------
+  uint32_t top = sizeof(K) == 2 ? KO::kEmpty * 0x10001u : KO::kEmpty;
+  const uint32_t empty = top;
+  // (NaN becomes -inf, the number a maximum with -inf returns)
+  auto clean = [&](uint4 r) {
+    return make_uint4(KO::max_word(r.x, empty), KO::max_word(r.y, empty),
+                      KO::max_word(r.z, empty), KO::max_word(r.w, empty));
+  };
+  auto vec_top = [](uint4 r) {
+    return KO::max_word(KO::max_word(r.x, r.y), KO::max_word(r.z, r.w));
+  };
+  constexpr int kAhead = 4;  // vectors a lane has in flight
+  for (int vb = v0 + lane; vb < v1; vb += 32 * kAhead) {
+    uint4 raw[kAhead];
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) k[j] = KO::key(e[j]);
-    } else {
-      const K *bits = reinterpret_cast<const K *>(src);
+    for (int a = 0; a < kAhead; ++a) {
+      const int v = vb + 32 * a, i0 = v * VEC - pad;  // first token of the vector
+      raw[a] = make_uint4(empty, empty, empty, empty);
+      if (v < v1) {
+        if (i0 >= 0 && i0 + VEC <= n) {
+          raw[a] = __ldcs(reinterpret_cast<const uint4 *>(src + i0));
+        } else {
+          const K *bits = reinterpret_cast<const K *>(src);
+          K *k = reinterpret_cast<K *>(&raw[a]);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        k[j] = (i0 + j >= 0 && i0 + j < n) ? KO::key(bits[i0 + j]) : K(0);
+          for (int j = 0; j < VEC; ++j)
+            if (i0 + j >= 0 && i0 + j < n) k[j] = bits[i0 + j];
+        }
+      }
     }
-    uint32_t kb = k[0];
-    int jb = 0;
 #pragma unroll
-    for (int j = 1; j < VEC; ++j)
-      if (k[j] > kb) kb = k[j], jb = j;
-    const u64 c = composite(kb, base + i0 + jb);
-    if (kb > KO::kNone && c > best) best = c;
-    *reinterpret_cast<uint4 *>(keys + v * VEC) = *reinterpret_cast<const uint4 *>(k);
+    for (int a = 0; a < kAhead; ++a) {
+      const uint4 r = clean(raw[a]);
+      top = KO::max_word(top, vec_top(r));
+      if (vb + 32 * a < v1) *reinterpret_cast<uint4 *>(keys + (vb + 32 * a) * VEC) = r;
+    }
   }
+  float best = KO::max_of(top);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const u64 y = __shfl_xor_sync(0xffffffffu, best, o);
-    best = y > best ? y : best;
-  }
-  if (lane == 0) sh.wsum[warp] = best;
+  for (int o = 16; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+  if (lane == 0) sh.dsum[warp] = best;
   __syncthreads();
   if (tid == 0) {
-    for (int i = 1; i < kSWarps; ++i) best = sh.wsum[i] > best ? sh.wsum[i] : best;
-    sh.maxc = best;
+    for (int i = 1; i < kSWarps; ++i) best = fmaxf(best, static_cast<float>(sh.dsum[i]));
+    sh.maxv = best;
   }
   cluster.sync();
-  u64 gmax = 0;
-  for (int r = 0; r < nrank; ++r) {
-    const u64 c = *cluster.map_shared_rank(&sh.maxc, r);
-    gmax = c > gmax ? c : gmax;
+  float xmax = -INFINITY;
+  for (int r = 0; r < nrank; ++r) xmax = fmaxf(xmax, *cluster.map_shared_rank(&sh.maxv, r));
+  const bool none = xmax == -INFINITY;
+  if (xmax == INFINITY) {  // the limit: +inf logits weigh the same, all others nothing
+    for (int v = v0 + lane; v < v1; v += 32) {
+      K *e = keys + v * VEC;
+      for (int j = 0; j < VEC; ++j) e[j] = KO::raw(e[j]) == INFINITY ? K(0) : KO::kEmpty;
+    }
+    __syncwarp();
+    xmax = 0.f;
   }
 
   const float temp = p.temperature ? p.temperature[row] : p.temperature_s;
@@ -285,61 +365,76 @@ __global__ void __launch_bounds__(kSThreads) sample_kernel(const SampleParams p)
   const bool greedy = !(temp > 0.f);
   const bool use_k = !greedy && top_k > 0 && top_k < p.vocab;
   const bool use_p = !greedy && top_p < 1.f;
-  const double minw = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) : 0.0;
+  // min-p on the scaled weights
+  const double minw = min_p > 0.f ? fmin(static_cast<double>(min_p), 1.0) * (1ull << kWeightBits)
+                                  : 0.0;
   RowW rw;
-  rw.fmax = KO::value(comp_key(gmax));
-  rw.xmax = rw.fmax;
-  rw.inv_t = greedy ? 1.0 : 1.0 / static_cast<double>(temp);
-  rw.fscale = static_cast<float>(8.0 * 1.4426950408889634 * rw.inv_t);
+  rw.fmax_ = xmax;
+  rw.xmax = xmax;
+  rw.c = greedy ? 1.0 : 1.4426950408889634 / static_cast<double>(temp);
+  // (finite and not 0: 0 * it is 0, and inf * it is inf)
+  rw.fscale = static_cast<float>(fmin(fmax(16.0 * rw.c, 1e-30), 3e38));
+  rw.table = sh.table;
 
-  // visits this thread's tokens (vectors of its warp in order): f(key, token)
-  auto each = [&](auto &&f) {
+  // Visits this thread's tokens above -inf (vectors of its warp in order):
+  // f(bits, logit, token). A vector whose largest logit pre() turns down is
+  // passed over: one test for VEC tokens, most of which no search is after.
+  auto each = [&](auto &&pre, auto &&f) {
     for (int v = v0 + lane; v < v1; v += 32) {
       const uint4 raw = *reinterpret_cast<const uint4 *>(keys + v * VEC);
+      if (!pre(KO::max_of(vec_top(raw)))) continue;
       const K *e = reinterpret_cast<const K *>(&raw);
       const int i0 = base + v * VEC - pad;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j)
-        if (e[j] > KO::kNone) f(static_cast<uint32_t>(e[j]), static_cast<uint32_t>(i0 + j));
+      for (int j = 0; j < VEC; ++j) {
+        const float x = KO::raw(e[j]);
+        if (x > -INFINITY) f(e[j], x, static_cast<uint32_t>(i0 + j));
+      }
     }
+  };
+  auto comp_of = [&](K bits, uint32_t i) { return composite(KO::key(bits), i); };
+  // one value per thread summed over the CTA in a fixed order; thread 0 has it
+  auto block_sum = [&](double d, double *part) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+    if (lane == 0) part[warp] = d;
+    __syncthreads();
+    if (tid == 0)
+      for (int i = 1; i < kSWarps; ++i) d += part[i];
+    return d;
   };
 
   // log-sum-exp of the row at temperature 1, for the log-probability
-  if (p.logprob && gmax != 0) {
+  if (p.logprob && !none) {
     float s = 0.f;
-    each([&](uint32_t k, uint32_t) {
-      const float x = KO::value(k);
-      s += x == rw.fmax ? 1.f : exp2f((x - rw.fmax) * kLog2e);
-    });
-    double d = s;
+    for (int v = v0 + lane; v < v1; v += 32) {
+      const uint4 raw = *reinterpret_cast<const uint4 *>(keys + v * VEC);
+      const K *e = reinterpret_cast<const K *>(&raw);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    double *part = reinterpret_cast<double *>(sh.scan);
-    if (lane == 0) part[warp] = d;
-    __syncthreads();
-    if (tid == 0) {
-      for (int i = 1; i < kSWarps; ++i) d += part[i];
-      sh.lsum = d;
+      for (int j = 0; j < VEC; ++j) s += fast_exp2((KO::raw(e[j]) - rw.fmax_) * kLog2e);
     }
-    __syncthreads();
+    const double d = block_sum(s, sh.dsum2);
+    if (tid == 0) sh.lsum = d;
   }
 
-  u64 thr = 0;        // tokens with a composite >= thr are kept
+  // the last token kept, once a search has found one (before: any above -inf)
+  Place thr{-INFINITY, 0};
+  bool cut = false;
+  auto place_of = [&](u64 c) { return Place{KO::value(comp_key(c)), comp_idx(c)}; };
   bool done = false;  // resolved on a list (by every CTA alike)
-  int sel = 0;        // threshold searches done (list_n buffer)
-  int level = 0;      // histogram levels done (hist buffer)
+  int sel = 0;        // this threshold search (fine, total and list_n buffers)
+  int level = 0;      // wide histogram levels done (hist buffer)
+  int listed = 0;     // tokens gathered
 
-  // Sums this level's histogram over the cluster and finds the first bin whose
-  // running sum reaches the target: results in r_u32 = {bin, count above, count
-  // in it}, r_u64 = {mass above, total mass, total count}. target < 0: the mass
-  // target is frac * total mass.
-  auto merge = [&](bool by_mass, double target, double frac, u64 have) {
-    cluster.sync();
-    Bin b{0, 0, 0, 0};
+  // Sums this level's histogram over the cluster (after its barrier) and finds
+  // the first bin whose running sum, past what lies above, reaches the target:
+  // r_u32 = {bin or kBins, count in earlier bins, count in it}, r_u64[0] = mass
+  // in earlier bins.
+  auto merge = [&](bool by_mass, double target, double above, u64 above_m) {
     u64 m = 0, c = 0;
     if (tid < kBins) {
       for (int r = 0; r < nrank; ++r) {
-        b = *cluster.map_shared_rank(&sh.hist[level & 1][tid], r);
+        const Bin b = *cluster.map_shared_rank(&sh.hist[level & 1][tid], r);
         c += b.n;
         m += static_cast<u64>(b.l0) + (static_cast<u64>(b.l1) << kLimb) +
              (static_cast<u64>(b.l2) << (2 * kLimb));
@@ -347,18 +442,14 @@ __global__ void __launch_bounds__(kSThreads) sample_kernel(const SampleParams p)
     }
     const u64 cs = block_scan(c, sh.scan);
     const u64 ms = by_mass ? block_scan(m, sh.scan) : 0;
-    if (tid == kSThreads - 1) {
-      sh.r_u64[1] = ms;
-      sh.r_u64[2] = cs;
-    }
     if (tid == 0) sh.r_u32[0] = kBins;
     __syncthreads();
-    if (by_mass && target < 0) target = frac * static_cast<double>(sh.r_u64[1]);
-    // the first bin that reaches the target; a prefix of at least one token
-    const double at = by_mass ? static_cast<double>(have + ms) : static_cast<double>(have + cs);
-    const double was = by_mass ? static_cast<double>(have + ms - m)
-                               : static_cast<double>(have + cs - c);
-    if (tid < kBins && c > 0 && at >= target && (was < target || cs == c)) {
+    const double at = by_mass ? static_cast<double>(above_m + ms) : above + static_cast<double>(cs);
+    const double was = by_mass ? static_cast<double>(above_m + ms - m)
+                               : above + static_cast<double>(cs - c);
+    // (nothing earlier anywhere: at least one token is kept)
+    const bool only = cs == c && (by_mass ? above_m == 0 : above == 0.0);
+    if (tid < kBins && c > 0 && at >= target && (was < target || only)) {
       sh.r_u32[0] = tid;
       sh.r_u32[1] = static_cast<uint32_t>(cs - c);
       sh.r_u32[2] = static_cast<uint32_t>(c);
@@ -366,10 +457,6 @@ __global__ void __launch_bounds__(kSThreads) sample_kernel(const SampleParams p)
     }
     __syncthreads();
     ++level;
-    // the next level's buffer: every CTA has read it before this barrier
-    if (tid < kBins) sh.hist[level & 1][tid] = Bin{0, 0, 0, 0};
-    __syncthreads();
-    return target;
   };
   auto add = [&](int b, bool by_mass, u64 w) {
     Bin *h = &sh.hist[level & 1][b];
@@ -383,85 +470,294 @@ __global__ void __launch_bounds__(kSThreads) sample_kernel(const SampleParams p)
   };
   // Gathers the tokens f accepts (at most kCap over the cluster), sorts them:
   // this thread's composite in descending order (0: none).
-  auto gather = [&](auto &&f) {
+  auto gather = [&](auto &&pre, auto &&f) {
     uint32_t *cnt = &sh.list_n[sel & 1];
-    each([&](uint32_t k, uint32_t i) {
-      const u64 c = composite(k, i);
-      if (f(k, c)) {
+    each(pre, [&](K bits, float x, uint32_t i) {
+      if (f(x, i)) {
         const uint32_t at = atomicAdd(cnt, 1u);
-        if (at < kCap) sh.list[at] = c;
+        if (at < kCap) sh.list[at] = comp_of(bits, i);
       }
     });
     cluster.sync();
-    u64 mine = 0;
-    uint32_t off = 0;
+    // this thread's entry of the ranks' lists, one after the other
+    int src_rank = -1;
+    uint32_t off = 0, at = 0;
     for (int r = 0; r < nrank; ++r) {
       const uint32_t m = min(*cluster.map_shared_rank(cnt, r), static_cast<uint32_t>(kCap));
-      if (tid >= off && tid < off + m) mine = *cluster.map_shared_rank(&sh.list[tid - off], r);
+      if (tid >= off && tid < off + m) src_rank = r, at = tid - off;
       off += m;
     }
-    ++sel;
-    return block_sort_desc(mine, sh.sorted);
+    const u64 mine = src_rank >= 0 ? *cluster.map_shared_rank(&sh.list[at], src_rank) : 0;
+    listed = min(off, static_cast<uint32_t>(kCap));
+    return mine;
   };
   auto weight_of = [&](u64 c) { return c ? rw.weight(KO::value(comp_key(c))) : 0ull; };
-
-  // ---- 2., 3. the filters' thresholds ---------------------------------------
-  const int nsel = (use_k ? 1 : 0) + (use_p ? 1 : 0);
-  for (int s = 0; s < nsel && gmax != 0 && !done; ++s) {
-    const bool by_mass = !(use_k && s == 0);
-    each([&](uint32_t k, uint32_t i) {
-      if (composite(k, i) < thr) return;
-      const float x = KO::value(k);
-      add(rw.bin(x), by_mass, by_mass ? rw.weight(x) : 0);
-    });
-    double target = merge(by_mass, by_mass ? -1.0 : static_cast<double>(top_k), top_p, 0);
-    const uint32_t b = sh.r_u32[0];
-    if (b == kBins) continue;  // fewer than k tokens: all are kept
-    uint32_t above = sh.r_u32[1], inside = sh.r_u32[2];
-    u64 above_m = sh.r_u64[0];
+  // Rank of this thread's listed token and the weight before it in the order.
+  auto place_in_list = [&](u64 c, u64 w, int *rank_out, u64 *before_out) {
+    if (tid < listed) sh.pairs[tid] = make_ulonglong2(c, w);
     __syncthreads();
-    if (above + inside <= kCap) {
-      // everything that may be kept fits the list
-      const u64 c = gather([&](uint32_t k, u64 c) {
-        return c >= thr && rw.bin(KO::value(k)) <= static_cast<int>(b);
-      });
-      u64 w = weight_of(c);
-      bool keep = c != 0;
-      if (!by_mass) keep = keep && tid < top_k;
-      if (use_p) {
-        const u64 upto = block_scan(keep ? w : 0, sh.scan);
-        if (tid == kSThreads - 1) sh.r_u64[3] = upto;
-        __syncthreads();
-        // (mass search: the target is a share of all the row's mass)
-        const double want = by_mass ? target : top_p * static_cast<double>(sh.r_u64[3]);
-        keep = keep && (tid == 0 || static_cast<double>(upto - w) < want);
+    int rk = 0;
+    u64 before = 0;
+    if (tid < listed) {
+#pragma unroll 4
+      for (int j = 0; j < listed; ++j) {
+        const ulonglong2 o = sh.pairs[j];
+        if (o.x > c) {
+          ++rk;
+          before += o.y;
+        }
       }
-      if (minw > 0.0) keep = keep && rw.weight_f(KO::value(comp_key(c))) >= minw;
-      // by index, weight in the low bits (18 + 45 bits); ~: ascending
-      const u64 packed =
-          keep ? ~((static_cast<u64>(comp_idx(c)) << (kWeightBits + 1)) | w) : 0ull;
-      const u64 sorted = block_sort_desc(packed, sh.sorted);
-      w = sorted ? (~sorted & ((1ull << (kWeightBits + 1)) - 1)) : 0;
-      const u64 cum = block_scan(w, sh.scan);
-      if (tid == kSThreads - 1) sh.r_u64[3] = cum;
+    }
+    *rank_out = rk;
+    *before_out = before;
+  };
+  // sh.acc[slot] += v over the CTA (integers: in any order)
+  auto accumulate = [&](u64 v, int slot) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0 && v) atomicAdd(&sh.acc[slot], v);
+  };
+  // Calls f(logit, token) for the tokens in(logit, token) accepts, whole warps at
+  // a time: few tokens of a row are, and a weight is some 40 instructions.
+  auto packed = [&](float least_x, auto &&in, auto &&f) {
+    float2 *q = sh.queue[warp];
+    int have = 0;
+    for (int vw = v0; vw < v1; vw += 32) {
+      uint4 raw = make_uint4(empty, empty, empty, empty);
+      if (vw + lane < v1) raw = *reinterpret_cast<const uint4 *>(keys + (vw + lane) * VEC);
+      const K *e = reinterpret_cast<const K *>(&raw);
+      const int i0 = base + (vw + lane) * VEC - pad;
+      if (!__any_sync(0xffffffffu, KO::max_of(vec_top(raw)) >= least_x)) continue;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float x = KO::raw(e[j]);
+        const bool mine = x > -INFINITY && in(x, static_cast<uint32_t>(i0 + j));
+        const uint32_t m = __ballot_sync(0xffffffffu, mine);
+        if (m == 0) continue;
+        if (mine)
+          q[have + __popc(m & ((1u << lane) - 1u))] = make_float2(x, __int_as_float(i0 + j));
+        have += __popc(m);
+        __syncwarp();
+        if (have >= 32) {
+          const float2 t = q[lane], rest = q[32 + lane];
+          __syncwarp();
+          have -= 32;
+          if (lane < have) q[lane] = rest;
+          __syncwarp();
+          f(t.x, __float_as_uint(t.y));
+        }
+      }
+    }
+    if (lane < have) f(q[lane].x, __float_as_uint(q[lane].y));
+    __syncwarp();
+  };
+
+  // ordered key of the largest logit (its float maps back to the type's bits)
+  auto key_of_max = [&]() -> uint32_t { return KO::key(KO::bits(rw.fmax_)); };
+  // ---- 2. to 4. the filters' thresholds ----------------------------------------
+  const int nsel = (use_k ? 1 : 0) + (use_p ? 1 : 0);
+  for (; sel < nsel && !none && !done; ++sel) {
+    const bool by_mass = !(use_k && sel == 0);
+    // -- 2. counts per bin, and the mass
+    uint32_t *fine = sh.fine[sel];
+    double sum = 0.0;
+    // weight at t sixteenths, for what lies below 2^-8 (t = inf: 0)
+    auto scaled_far = [](float t) {
+      return fast_exp2(fmaf(t, -0.0625f, static_cast<float>(kWeightBits)));
+    };
+    auto count = [&](float z) { atomicAdd(&fine[__float_as_uint(z) & (kFine - 1)], 1u); };
+    for (int v = v0 + lane; v < v1; v += 32) {
+      const uint4 raw = *reinterpret_cast<const uint4 *>(keys + v * VEC);
+      const K *e = reinterpret_cast<const K *>(&raw);
+      const float t0 = rw.steps(KO::max_of(vec_top(raw)));  // the vector's least
+      if (t0 + kRound <= kRound + (kNear - 1)) {
+        float far = 0.f, t[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          t[j] = rw.steps(KO::raw(e[j]));
+          if (cut && !thr.takes(KO::raw(e[j]), base + v * VEC - pad + j)) t[j] = INFINITY;
+          const float z = t[j] + kRound;
+          if (z <= kRound + (kNear - 1)) count(z);
+          if (by_mass) far += t[j] >= kExact ? scaled_far(t[j]) : 0.f;
+        }
+        if (by_mass) {
+          sum += far;
+          if (t0 < kExact) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+              const double w = rw.scaled(KO::raw(e[j]));
+              sum += t[j] < kExact ? w : 0.0;
+            }
+          }
+        }
+      } else if (by_mass) {
+        float far = 0.f;
+        if (cut) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j)
+            if (thr.takes(KO::raw(e[j]), base + v * VEC - pad + j))
+              far += scaled_far(rw.steps(KO::raw(e[j])));
+        } else {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) far += scaled_far(rw.steps(KO::raw(e[j])));
+        }
+        sum += far;
+      }
+    }
+    if (by_mass) {
+      const double d = block_sum(sum, sh.dsum);
+      if (tid == 0) sh.total[sel] = d;
+    }
+    double target = top_k, total = 0.0;
+    int fb = kFine, fa = kFine;
+    uint32_t above_n = 0, upto_n = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+      if (pass) {  // undecided: the other bins
+        for (int v = v0 + lane; v < v1; v += 32) {
+          const uint4 raw = *reinterpret_cast<const uint4 *>(keys + v * VEC);
+          const K *e = reinterpret_cast<const K *>(&raw);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const float x = KO::raw(e[j]), z = rw.steps(x) + kRound;
+            if (z > kRound + (kNear - 1) && z <= kRound + (kFine - 1) &&
+                (!cut || thr.takes(x, base + v * VEC - pad + j)))
+              count(z);
+          }
+        }
+      }
+      cluster.sync();
+      if (by_mass && pass == 0) {
+        for (int r = 0; r < nrank; ++r) total += *cluster.map_shared_rank(&sh.total[sel], r);
+        target = total * top_p;
+      }
+      // The first bin by which the prefix has certainly reached the target (fb),
+      // and the first by which it may have (fa): exact for counts; by mass the
+      // prefix lies between its counts times the bins' least and most weights,
+      // and, once all bins are counted, between the whole mass less the rest's
+      // most and least weights (1e-4: the roundings of t, exp2f, fp32 sums and
+      // what lies past the bins). Thread t has bins 2 t and 2 t + 1.
+      uint32_t c0 = 0, c1 = 0;
+      if (pass || tid < kNear / 2) {
+        for (int r = 0; r < nrank; ++r) {
+          const uint2 x =
+              *cluster.map_shared_rank(reinterpret_cast<const uint2 *>(sh.fine[sel]) + tid, r);
+          c0 += x.x;
+          c1 += x.y;
+        }
+      }
+      constexpr float kLeast = 0.95760328f;  // 2^(-1/16): a bin's least weight over its most
+      const float top = by_mass ? fast_exp2(-0.0625f * (2 * tid - 0.5f) + kWeightBits) : 0.f;
+      const float h0 = c0 * top, h1 = c1 * (top * kLeast);
+      uint32_t n_in = c0 + c1;
+      float hi_in = h0 + h1;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, n_in, o);
+        const float z = __shfl_up_sync(0xffffffffu, hi_in, o);
+        if (lane >= o) {
+          n_in += y;
+          hi_in += z;
+        }
+      }
+      if (lane == 31) {
+        sh.warp_n[warp] = n_in;
+        sh.warp_hi[warp] = hi_in;
+      }
+      if (tid == 0) sh.r_u32[0] = sh.r_u32[2] = kFine;
       __syncthreads();
-      const u64 at = static_cast<u64>(static_cast<double>(u) * static_cast<double>(sh.r_u64[3]));
-      if (w && cum > at && cum - w <= at)
-        sh.token = static_cast<int>((~sorted >> (kWeightBits + 1)) & kIdxMask);
+      uint32_t n_all = 0;
+      float hi_all = 0.f;
+#pragma unroll
+      for (int i = 0; i < kSWarps; ++i) {
+        if (i == warp) {
+          n_in += n_all;
+          hi_in += hi_all;
+        }
+        n_all += sh.warp_n[i];
+        hi_all += sh.warp_hi[i];
+      }
+      const uint32_t n0 = n_in - c1;  // up to bin 2 t
+      bool fb0, fb1, fa0, fa1;
+      if (by_mass) {
+        const float whole = static_cast<float>(total), goal = static_cast<float>(target);
+        const float rest = pass ? hi_all : INFINITY, hi0 = hi_in - h1, slack = 1e-4f * whole;
+        fb0 = fmaxf(hi0 * kLeast, whole - (rest - hi0)) - slack >= goal;
+        fb1 = fmaxf(hi_in * kLeast, whole - (rest - hi_in)) - slack >= goal;
+        fa0 = (pass ? fminf(hi0, whole - (rest - hi0) * kLeast) : hi0) + slack >= goal;
+        fa1 = (pass ? fminf(hi_in, whole - (rest - hi_in) * kLeast) : hi_in) + slack >= goal;
+      } else {
+        fb0 = fa0 = n0 >= static_cast<uint32_t>(top_k);
+        fb1 = fa1 = n_in >= static_cast<uint32_t>(top_k);
+      }
+      // (a bin before the first token's does not count: one token is always kept)
+      const int b0 = n0 > 0 ? 2 * tid : 2 * tid + 1;
+      if (n_in > 0 && (fb0 || fb1)) atomicMin(&sh.r_u32[0], fb0 ? b0 : 2 * tid + 1);
+      if (n_in > 0 && (fa0 || fa1)) atomicMin(&sh.r_u32[2], fa0 ? b0 : 2 * tid + 1);
+      __syncthreads();
+      fb = static_cast<int>(sh.r_u32[0]), fa = static_cast<int>(sh.r_u32[2]);
+      if (tid == fb >> 1) sh.r_u32[1] = fb & 1 ? n_in : n0;
+      if (tid == min(fa, kFine - 1) >> 1)  // the count above bin fa
+        sh.r_u32[3] = fa == kFine ? n_in : (fa & 1 ? n0 : n0 - c0);
+      __syncthreads();
+      upto_n = sh.r_u32[1], above_n = sh.r_u32[3];
+      if (fb < kNear) break;
+      __syncthreads();
+    }
+    // fewer than k tokens down to 2^-64: what lies below is never drawn
+    if (!by_mass && fb == kFine) continue;
+    if (fb < kFine && upto_n <= kCap) {
+      // -- 3. everything that may be kept fits the list
+      const u64 c = gather([&](float x) { return rw.within(x, fb); },
+                           [&](float x, uint32_t i) {
+                             return rw.within(x, fb) && (!cut || thr.takes(x, i));
+                           });
+      const u64 w = weight_of(c);
+      int rk;
+      u64 before;
+      place_in_list(c, w, &rk, &before);
+      bool keep = c != 0 && (by_mass || rk < top_k);
+      if (use_p) {
+        // (mass search: the target is a share of all the row's mass)
+        double want = target;
+        if (!by_mass) {
+          accumulate(keep ? w : 0, 0);
+          __syncthreads();
+          want = top_p * static_cast<double>(sh.acc[0]);
+        }
+        keep = keep && (rk == 0 || static_cast<double>(before) < want);
+      }
+      if (minw > 0.0) keep = keep && rw.scaled(KO::value(comp_key(c))) >= minw;
+      accumulate(keep ? w : 0, 1);
+      __syncthreads();  // (also: the list has been read)
+      if (tid < listed) sh.pairs[tid].y = keep ? w : 0;
+      __syncthreads();
+      if (keep) {  // mass of the kept tokens with a lower index
+        const u64 at = static_cast<u64>(static_cast<double>(u) * static_cast<double>(sh.acc[1]));
+        const uint32_t low = static_cast<uint32_t>(c) & kIdxMask;
+        u64 cum = 0;
+#pragma unroll 4
+        for (int j = 0; j < listed; ++j) {
+          const ulonglong2 o = sh.pairs[j];
+          if ((static_cast<uint32_t>(o.x) & kIdxMask) > low) cum += o.y;
+        }
+        if (cum <= at && at < cum + w) sh.token = static_cast<int>(comp_idx(c));
+      }
       __syncthreads();
       done = true;
       break;
     }
-    // the range of composites that bin b holds: its keys by a 32-way search
-    // (bin() falls as the key grows), the same in every warp
+    // -- 4. wide: the range of composites of bins fa to fb, or to the row's end;
+    // its keys by a 32-way search (bins fall as the key grows), alike in every warp
+    __syncthreads();
     u64 lo, hi;
     {
+      const uint32_t kmax = key_of_max();
       auto edge = [&](int limit) {  // smallest key above kNone with bin <= limit
-        uint32_t l = KO::kNone + 1, h = comp_key(gmax);  // the answer is in [l, h]
+        uint32_t l = KO::kNone + 1, h = kmax;  // the answer is in [l, h]
         while (l < h) {
           const uint32_t step = (h - l + 31) / 32;
           const u64 at = static_cast<u64>(l) + static_cast<u64>(step) * lane;
-          const bool in = at >= h || rw.bin(KO::value(static_cast<uint32_t>(at))) <= limit;
+          const bool in = at >= h || rw.within(KO::value(static_cast<uint32_t>(at)), limit);
           const uint32_t m = __ballot_sync(0xffffffffu, in);
           const int first = m ? __ffs(m) - 1 : 32;
           const u64 nl = first ? static_cast<u64>(l) + static_cast<u64>(step) * (first - 1) + 1 : l;
@@ -473,74 +769,162 @@ __global__ void __launch_bounds__(kSThreads) sample_kernel(const SampleParams p)
         }
         return l;
       };
-      const uint32_t klo = edge(static_cast<int>(b));
-      const uint32_t khi = b == 0 ? comp_key(gmax) : edge(static_cast<int>(b) - 1) - 1;
+      const uint32_t klo = fb < kFine ? edge(fb) : KO::kNone + 1;
+      const uint32_t khi = fa == 0 ? kmax : edge(fa - 1) - 1;
       lo = static_cast<u64>(klo) << kIdxBits;
       hi = (static_cast<u64>(khi) << kIdxBits) | kIdxMask;
-      if (lo < thr) lo = thr;
+      if (cut) lo = max(lo, composite(KO::key(KO::bits(thr.x)), thr.i));
     }
-    // divide the range until its tokens fit the list
-    while (inside > kCap) {
+    if (lo > hi) continue;  // no token past the bins: all are kept
+    // divide the range until its tokens fit the list; the first time also the
+    // mass above it (the count above is known)
+    u64 above_m = 0;
+    double above = above_n;
+    bool all = false;  // the target is not reached: everything in the range is kept
+    for (uint32_t inside = UINT32_MAX; inside > kCap;) {
       const int shift = max(0, 64 - __clzll(static_cast<long long>(hi - lo)) - 8);
-      each([&](uint32_t k, uint32_t i) {
-        const u64 c = composite(k, i);
-        if (c >= lo && c <= hi)
-          add(static_cast<int>((hi - c) >> shift), by_mass, by_mass ? rw.weight(KO::value(k)) : 0);
-      });
-      merge(by_mass, target, 0.0, by_mass ? above_m : above);
+      for (int i = tid; i < kBins; i += kSThreads) sh.hist[level & 1][i] = Bin{0, 0, 0, 0};
+      __syncthreads();
+      u64 over = 0;
+      const bool first = inside == UINT32_MAX;
+      const Place least = place_of(lo), most = place_of(hi + 1);  // range: takes least, not most
+      packed(
+          least.x,
+          [&](float x, uint32_t i) {
+            return least.takes(x, i) && ((by_mass && first) || !most.takes(x, i));
+          },
+          [&](float x, uint32_t i) {
+            const u64 w = by_mass ? rw.weight(x) : 0;
+            if (most.takes(x, i))
+              over += w;
+            else
+              add(static_cast<int>((hi - comp_of(KO::bits(x), i)) >> shift), by_mass, w);
+          });
+      if (by_mass && first) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) over += __shfl_xor_sync(0xffffffffu, over, o);
+        if (lane == 0) sh.wsum[warp] = over;
+        __syncthreads();
+        if (tid == 0) {
+          for (int i = 1; i < kSWarps; ++i) over += sh.wsum[i];
+          sh.over = over;
+        }
+      }
+      cluster.sync();
+      if (by_mass && first) {
+        for (int r = 0; r < nrank; ++r) above_m += *cluster.map_shared_rank(&sh.over, r);
+        above = static_cast<double>(above_m);
+      }
+      merge(by_mass, target, above, above_m);
       const uint32_t q = sh.r_u32[0];
-      above += sh.r_u32[1];
+      if (q == kBins) {
+        all = true;
+        break;
+      }
+      above += sh.r_u32[1];  // (counts; by mass it is above_m that counts)
       inside = sh.r_u32[2];
       above_m += sh.r_u64[0];
+      if (by_mass) above = static_cast<double>(above_m);
       __syncthreads();
       hi -= static_cast<u64>(q) << shift;
       const u64 width = (1ull << shift) - 1;
       if (hi - lo > width) lo = hi - width;
     }
-    const u64 c = gather([&](uint32_t, u64 c) { return c >= lo && c <= hi; });
-    u64 w = by_mass ? weight_of(c) : (c ? 1 : 0);
-    const u64 upto = (by_mass ? above_m : above) + block_scan(w, sh.scan);
+    if (all) {
+      thr = place_of(lo);
+      cut = true;
+      __syncthreads();
+      continue;
+    }
+    const Place least = place_of(lo), most = place_of(hi + 1);
+    const u64 gc = gather(
+        [&](float x) { return x >= least.x; },
+        [&](float x, uint32_t i) { return least.takes(x, i) && !most.takes(x, i); });
+    const u64 w = by_mass ? weight_of(gc) : (gc ? 1 : 0);
+    int rk;
+    u64 before;
+    place_in_list(gc, w, &rk, &before);
+    before += by_mass ? above_m : static_cast<u64>(above);
     // the last kept: the first whose running sum reaches the target
-    if (c && static_cast<double>(upto) >= target &&
-        (tid == 0 || static_cast<double>(upto - w) < target))
-      sh.r_u64[3] = c;
+    if (gc && static_cast<double>(before + w) >= target &&
+        (static_cast<double>(before) < target || before == 0))
+      sh.r_u64[3] = gc;
     __syncthreads();
-    thr = sh.r_u64[3];
+    thr = place_of(sh.r_u64[3]);
+    cut = true;
     __syncthreads();
   }
 
-  // ---- 4. the draw ------------------------------------------------------------
-  auto finish = [&](uint32_t key, int token) {  // one thread of the cluster
+  // ---- the draw -----------------------------------------------------------------
+  auto finish = [&](float x, int token) {  // one thread of the cluster
     p.out[row] = token;
     if (p.logprob) {
       double s = 0;
       for (int r = 0; r < nrank; ++r) s += *cluster.map_shared_rank(&sh.lsum, r);
-      const float x = KO::value(key);
-      const double d = x == rw.fmax ? 0.0 : static_cast<double>(x) - rw.xmax;
+      const double d = x == rw.fmax_ ? 0.0 : static_cast<double>(x) - rw.xmax;
       p.logprob[row] = static_cast<float>(d - log(s));
     }
   };
-  if (gmax == 0) {  // no finite or +inf logit
+  if (none) {  // no logit above -inf
     if (rank == 0 && tid == 0) {
       p.out[row] = -1;
       if (p.logprob) p.logprob[row] = -INFINITY;
       flag(p.status, MI_STATUS_NO_TOKEN);
     }
   } else if (greedy) {
-    if (p.logprob) cluster.sync();  // every CTA's lsum is written
-    if (rank == 0 && tid == 0) finish(comp_key(gmax), static_cast<int>(comp_idx(gmax)));
+    uint32_t first = 0xFFFFFFFFu;
+    each([&](float x) { return x == rw.fmax_; },
+         [&](K, float x, uint32_t i) {
+           if (x == rw.fmax_) first = min(first, i);
+         });
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (lane == 0) atomicMin(&sh.first, first);
+    cluster.sync();  // (every CTA's lsum is written, too)
+    if (rank == 0 && tid == 0) {
+      for (int r = 0; r < nrank; ++r)
+        first = min(first, *cluster.map_shared_rank(&sh.first, r));
+      finish(rw.fmax_, static_cast<int>(first));
+    }
   } else if (done) {
-    // the CTA that holds the token has its key
+    // the CTA that holds the token has its logit
     const int t = sh.token;
-    if (tid == 0 && t >= base && t < base + n) finish(keys[t - base + pad], t);
+    if (tid == 0 && t >= base && t < base + n) finish(KO::raw(keys[t - base + pad]), t);
   } else {
-    auto kept = [&](uint32_t k, uint32_t i) {
-      if (composite(k, i) < thr) return 0ull;
-      const double e = rw.weight_f(KO::value(k));
-      return e >= minw ? __double2ull_rn(e * static_cast<double>(1ull << kWeightBits)) : 0ull;
+    // kept weights of a vector's tokens (0: not kept); any: some lane has one
+    auto kept = [&](const K *e, int i0, u64 *w) {
+      bool in[VEC], some = false;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float x = KO::raw(e[j]);
+        in[j] = x > -INFINITY && (!cut || thr.takes(x, i0 + j));
+        some = some || in[j];
+      }
+      if (!__any_sync(0xffffffffu, some)) return false;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const double d = rw.scaled(KO::raw(e[j]));
+        w[j] = in[j] && d >= minw ? RowW::whole(d) : 0ull;
+      }
+      return true;
     };
     u64 m = 0;
-    each([&](uint32_t k, uint32_t i) { m += kept(k, i); });
+    if (cut) {
+      packed(thr.x, [&](float x, uint32_t i) { return thr.takes(x, i); },
+             [&](float x, uint32_t) {
+               const double d = rw.scaled(x);
+               m += d >= minw ? RowW::whole(d) : 0ull;
+             });
+    } else {  // all tokens: no need to pack
+      for (int vw = v0; vw < v1; vw += 32) {
+        uint4 raw = make_uint4(empty, empty, empty, empty);
+        if (vw + lane < v1) raw = *reinterpret_cast<const uint4 *>(keys + (vw + lane) * VEC);
+        u64 w[VEC];
+        if (kept(reinterpret_cast<const K *>(&raw), base + (vw + lane) * VEC - pad, w)) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) m += w[j];
+        }
+      }
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
     if (lane == 0) sh.wsum[warp] = m;
@@ -566,14 +950,14 @@ __global__ void __launch_bounds__(kSThreads) sample_kernel(const SampleParams p)
       if (warp == ww) {
         u64 run = wb;
         for (int v = v0; v < v1; v += 32) {
-          uint4 raw = make_uint4(0, 0, 0, 0);
+          uint4 raw = make_uint4(empty, empty, empty, empty);
           if (v + lane < v1) raw = *reinterpret_cast<const uint4 *>(keys + (v + lane) * VEC);
           const K *e = reinterpret_cast<const K *>(&raw);
           const int i0 = base + (v + lane) * VEC - pad;
-          u64 mine = 0;
+          u64 w[VEC], mine = 0;
+          if (!kept(e, i0, w)) continue;
 #pragma unroll
-          for (int j = 0; j < VEC; ++j)
-            if (e[j] > KO::kNone) mine += kept(e[j], i0 + j);
+          for (int j = 0; j < VEC; ++j) mine += w[j];
           u64 incl = mine;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
@@ -584,14 +968,14 @@ __global__ void __launch_bounds__(kSThreads) sample_kernel(const SampleParams p)
           if (at < run + sum) {
             u64 c = run + incl - mine;
             if (at >= c && at < c + mine) {
+              bool open = true;
+#pragma unroll
               for (int j = 0; j < VEC; ++j) {
-                if (e[j] <= KO::kNone) continue;
-                const u64 w = kept(e[j], i0 + j);
-                if (at < c + w) {
-                  finish(e[j], i0 + j);
-                  break;
+                if (open && at < c + w[j]) {
+                  finish(KO::raw(e[j]), i0 + j);
+                  open = false;
                 }
-                c += w;
+                c += w[j];
               }
             }
             break;
