@@ -23,7 +23,7 @@
 //      or above which everything that may be kept lies: token counts for
 //      top-k; for top-p counts times each bin's least or most weight, against
 //      p times the row's mass. Only the tokens within 2^-16 of the largest
-//      weight are counted at first (most of a row's are not, and an atomic a
+//      weight (for top-k, within 12 of the largest logit) are counted at first (most of a row's are not, and an atomic a
 //      token would be the kernel's largest cost); where that does not decide,
 //      a second pass counts down to 2^-64 (nothing below 2^-45 can be drawn).
 //      The mass is summed in the same pass, with the exact 64-bit exponential
@@ -31,9 +31,10 @@
 //      little is as good;
 //   3. if no more than kCap tokens lie at or above that bin (the usual case),
 //      they are gathered, one per thread, and every filter and the draw happen
-//      on that list with exact weights: a thread finds its token's rank and the
-//      mass before it by comparing with all others (tens of tokens as a rule;
-//      sorting needs more barriers than that takes);
+//      on that list with exact weights, each as a search for the token at which
+//      a running sum crosses its target: by comparing with all others (tens of
+//      tokens as a rule; sorting needs more barriers than that takes), on a long
+//      list with those of the same 128th only;
 //   4. else ("wide" sets) the histogram brackets the bin where the prefix ends
 //      (exactly for counts; for masses between the bins' least and most
 //      weights), and divisions of the bracket's range of composites by 256,
@@ -45,6 +46,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "mi_common.cuh"
 #include "umma.cuh"
@@ -63,7 +65,9 @@ constexpr int kIdxBits = 18;     // vocabulary <= 2^18
 constexpr uint32_t kIdxMask = (1u << kIdxBits) - 1;
 constexpr int kWeightBits = 44;  // the largest weight is 2^44
 constexpr int kFine = 1024;      // bins of 1/16 of -log2 w (two per thread)
-constexpr int kNear = 256;       // the bins of the first pass: down to 2^-16
+constexpr int kNear = 256;       // bins of the first pass by mass: down to 2^-16
+constexpr float kNearX = 12.f;   // logits below the largest that it counts for top-k, at least
+constexpr int kShort = 128;      // lists up to this are searched as one
 constexpr float kExact = 128.f;  // exact weights down to 2^-8
 constexpr float kRound = 8388608.f;  // adding it rounds to an integer, in the low bits
 constexpr int kLimb = 15;        // histogram masses: three 15-bit limbs in 32-bit counters
@@ -217,11 +221,15 @@ struct __align__(16) Bin {
 struct Shared {
   double table[32];
   uint32_t fine[2][kFine];  // one buffer per search
-  Bin hist[2][kBins];
+  union {  // a list is searched after the last read of any histogram
+    Bin hist[2][kBins];
+    ulonglong2 pairs[kCap];         // entries of the gathered list: order, weight
+  };
   u64 list[kCap];   // this CTA's gathered composites
-  ulonglong2 pairs[kCap];           // the gathered list: composite, weight
   float2 queue[kSWarps][64];        // per warp: tokens waiting for their weight
-  u64 acc[4];                       // integer sums over the list
+  u64 share[128];                   // a long list's sums per 128th
+  u64 acc[4];                       // integer sums over the list; [3]: entries in pairs
+  u64 cross;
   u64 scan[kSWarps];
   uint32_t warp_n[kSWarps];
   float warp_hi[kSWarps];
@@ -230,7 +238,7 @@ struct Shared {
   // read by the other CTAs of the cluster, each written once before a barrier
   float maxv;
   double lsum;       // sum of exp(x - max), temperature 1
-  double total[2];   // mass, per search
+  double2 total[2];  // mass, and what of it the first pass counts, per search
   u64 mass, over;
   uint32_t first;    // lowest token with the largest logit
   uint32_t list_n[2];
@@ -344,8 +352,19 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
     sh.maxv = best;
   }
   cluster.sync();
+  // f(rank, that CTA's *field), four loads in flight together
+  auto ranks = [&](auto *field, auto &&f) {
+    for (int r0 = 0; r0 < nrank; r0 += 4) {
+      std::remove_reference_t<decltype(*field)> v[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = *cluster.map_shared_rank(field, min(r0 + r, nrank - 1));
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r0 + r < nrank) f(r0 + r, v[r]);
+    }
+  };
   float xmax = -INFINITY;
-  for (int r = 0; r < nrank; ++r) xmax = fmaxf(xmax, *cluster.map_shared_rank(&sh.maxv, r));
+  ranks(&sh.maxv, [&](int, float v) { xmax = fmaxf(xmax, v); });
   const bool none = xmax == -INFINITY;
   if (xmax == INFINITY) {  // the limit: +inf logits weigh the same, all others nothing
     for (int v = v0 + lane; v < v1; v += 32) {
@@ -432,14 +451,12 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
   // in earlier bins.
   auto merge = [&](bool by_mass, double target, double above, u64 above_m) {
     u64 m = 0, c = 0;
-    if (tid < kBins) {
-      for (int r = 0; r < nrank; ++r) {
-        const Bin b = *cluster.map_shared_rank(&sh.hist[level & 1][tid], r);
-        c += b.n;
-        m += static_cast<u64>(b.l0) + (static_cast<u64>(b.l1) << kLimb) +
-             (static_cast<u64>(b.l2) << (2 * kLimb));
-      }
-    }
+    if (tid < kBins)
+      ranks(reinterpret_cast<uint4 *>(&sh.hist[level & 1][tid]), [&](int, uint4 b) {
+        c += b.x;  // a Bin
+        m += static_cast<u64>(b.y) + (static_cast<u64>(b.z) << kLimb) +
+             (static_cast<u64>(b.w) << (2 * kLimb));
+      });
     const u64 cs = block_scan(c, sh.scan);
     const u64 ms = by_mass ? block_scan(m, sh.scan) : 0;
     if (tid == 0) sh.r_u32[0] = kBins;
@@ -482,34 +499,75 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
     // this thread's entry of the ranks' lists, one after the other
     int src_rank = -1;
     uint32_t off = 0, at = 0;
-    for (int r = 0; r < nrank; ++r) {
-      const uint32_t m = min(*cluster.map_shared_rank(cnt, r), static_cast<uint32_t>(kCap));
+    ranks(cnt, [&](int r, uint32_t m) {
+      m = min(m, static_cast<uint32_t>(kCap));
       if (tid >= off && tid < off + m) src_rank = r, at = tid - off;
       off += m;
-    }
+    });
     const u64 mine = src_rank >= 0 ? *cluster.map_shared_rank(&sh.list[at], src_rank) : 0;
     listed = min(off, static_cast<uint32_t>(kCap));
     return mine;
   };
   auto weight_of = [&](u64 c) { return c ? rw.weight(KO::value(comp_key(c))) : 0ull; };
-  // Rank of this thread's listed token and the weight before it in the order.
-  auto place_in_list = [&](u64 c, u64 w, int *rank_out, u64 *before_out) {
-    if (tid < listed) sh.pairs[tid] = make_ulonglong2(c, w);
+  // The listed token at which the running sum of w, from `above` on and in
+  // falling `order`, reaches the target (always one: the first, if none is
+  // needed): its order. part: the entry's 128th, rising as the order falls.
+  auto crossing = [&](bool has, u64 order, u64 w, uint32_t part, u64 above, double target) {
+    const bool shorts = listed <= kShort;
+    __syncthreads();  // (an earlier call's result has been read)
+    if (tid < 128) sh.share[tid] = 0;
+    if (tid == 0) {
+      sh.acc[3] = 0;
+      sh.cross = 0;
+      sh.r_u32[0] = 0;
+      sh.r_u64[0] = above;
+    }
     __syncthreads();
-    int rk = 0;
-    u64 before = 0;
-    if (tid < listed) {
-#pragma unroll 4
-      for (int j = 0; j < listed; ++j) {
-        const ulonglong2 o = sh.pairs[j];
-        if (o.x > c) {
-          ++rk;
-          before += o.y;
+    if (!shorts) {
+      if (has) atomicAdd(&sh.share[part], w);
+      __syncthreads();
+      if (warp == 0) {  // four parts a lane
+        u64 v[4], sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum += v[i] = sh.share[lane * 4 + i];
+        u64 run = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 y = shfl_up64(run, o);
+          if (lane >= o) run += y;
+        }
+        run += above - sum;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool first = run == 0;  // (nothing before it)
+          if (v[i] && static_cast<double>(run + v[i]) >= target &&
+              (first || static_cast<double>(run) < target)) {
+            sh.r_u32[0] = lane * 4 + i;
+            sh.r_u64[0] = run;
+          }
+          run += v[i];
         }
       }
+      __syncthreads();
+      has = has && part == sh.r_u32[0];
     }
-    *rank_out = rk;
-    *before_out = before;
+    if (has) sh.pairs[atomicAdd(reinterpret_cast<uint32_t *>(&sh.acc[3]), 1u)] =
+        make_ulonglong2(order, w);
+    __syncthreads();
+    if (has) {
+      const int m = static_cast<int>(sh.acc[3]);
+      u64 before = sh.r_u64[0];
+#pragma unroll 4
+      for (int j = 0; j < m; ++j) {
+        const ulonglong2 o = sh.pairs[j];
+        if (o.x > order) before += o.y;
+      }
+      if (w && static_cast<double>(before + w) >= target &&
+          (before == 0 || static_cast<double>(before) < target))
+        sh.cross = order;
+    }
+    __syncthreads();
+    return sh.cross;
   };
   // sh.acc[slot] += v over the CTA (integers: in any order)
   auto accumulate = [&](u64 v, int slot) {
@@ -561,54 +619,63 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
     // -- 2. counts per bin, and the mass
     uint32_t *fine = sh.fine[sel];
     double sum = 0.0;
+    float inside = 0.f;  // of the sum: what is counted, to fp32
     // weight at t sixteenths, for what lies below 2^-8 (t = inf: 0)
-    auto scaled_far = [](float t) {
+    auto far = [](float t) {
       return fast_exp2(fmaf(t, -0.0625f, static_cast<float>(kWeightBits)));
     };
     auto count = [&](float z) { atomicAdd(&fine[__float_as_uint(z) & (kFine - 1)], 1u); };
+    const int window =
+        by_mass ? kNear
+                : max(kNear, static_cast<int>(fminf(kNearX * rw.fscale, kFine - 2.f)) & ~1);
     for (int v = v0 + lane; v < v1; v += 32) {
       const uint4 raw = *reinterpret_cast<const uint4 *>(keys + v * VEC);
       const K *e = reinterpret_cast<const K *>(&raw);
       const float t0 = rw.steps(KO::max_of(vec_top(raw)));  // the vector's least
-      if (t0 + kRound <= kRound + (kNear - 1)) {
-        float far = 0.f, t[VEC];
+      const bool near = t0 + kRound <= kRound + (window - 1);
+      if (!near && !by_mass) continue;
+      float t[VEC], w[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          t[j] = rw.steps(KO::raw(e[j]));
-          if (cut && !thr.takes(KO::raw(e[j]), base + v * VEC - pad + j)) t[j] = INFINITY;
-          const float z = t[j] + kRound;
-          if (z <= kRound + (kNear - 1)) count(z);
-          if (by_mass) far += t[j] >= kExact ? scaled_far(t[j]) : 0.f;
-        }
-        if (by_mass) {
-          sum += far;
-          if (t0 < kExact) {
+      for (int j = 0; j < VEC; ++j) t[j] = rw.steps(KO::raw(e[j]));
+      if (cut) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              const double w = rw.scaled(KO::raw(e[j]));
-              sum += t[j] < kExact ? w : 0.0;
-            }
+        for (int j = 0; j < VEC; ++j)
+          if (!thr.takes(KO::raw(e[j]), base + v * VEC - pad + j)) t[j] = INFINITY;
+      }
+      if (by_mass) {
+        float part = 0.f;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) w[j] = far(t[j]);
+        if (t0 < kExact) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const double x = rw.scaled(KO::raw(e[j]));
+            sum += t[j] < kExact ? x : 0.0;
+            part += t[j] < kExact ? 0.f : w[j];
           }
-        }
-      } else if (by_mass) {
-        float far = 0.f;
-        if (cut) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j)
-            if (thr.takes(KO::raw(e[j]), base + v * VEC - pad + j))
-              far += scaled_far(rw.steps(KO::raw(e[j])));
         } else {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) far += scaled_far(rw.steps(KO::raw(e[j])));
+          for (int j = 0; j < VEC; ++j) part += w[j];
         }
-        sum += far;
+        sum += part;
+      }
+      if (near) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float z = t[j] + kRound;
+          if (z <= kRound + (window - 1)) {
+            count(z);
+            if (by_mass) inside += w[j];
+          }
+        }
       }
     }
     if (by_mass) {
-      const double d = block_sum(sum, sh.dsum);
-      if (tid == 0) sh.total[sel] = d;
+      const double d = block_sum(sum, sh.dsum), in = block_sum(inside, sh.dsum2);
+      if (tid == 0) sh.total[sel] = make_double2(d, in);
     }
     double target = top_k, total = 0.0;
+    float beyond = 0.f;  // mass not counted
     int fb = kFine, fa = kFine;
     uint32_t above_n = 0, upto_n = 0;
     for (int pass = 0; pass < 2; ++pass) {
@@ -619,7 +686,7 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
             const float x = KO::raw(e[j]), z = rw.steps(x) + kRound;
-            if (z > kRound + (kNear - 1) && z <= kRound + (kFine - 1) &&
+            if (z > kRound + (window - 1) && z <= kRound + (kFine - 1) &&
                 (!cut || thr.takes(x, base + v * VEC - pad + j)))
               count(z);
           }
@@ -627,24 +694,25 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
       }
       cluster.sync();
       if (by_mass && pass == 0) {
-        for (int r = 0; r < nrank; ++r) total += *cluster.map_shared_rank(&sh.total[sel], r);
+        double in = 0.0;
+        ranks(&sh.total[sel], [&](int, double2 v) {
+          total += v.x;
+          in += v.y;
+        });
         target = total * top_p;
+        beyond = static_cast<float>(total - in);
       }
       // The first bin by which the prefix has certainly reached the target (fb),
       // and the first by which it may have (fa): exact for counts; by mass the
       // prefix lies between its counts times the bins' least and most weights,
-      // and, once all bins are counted, between the whole mass less the rest's
-      // most and least weights (1e-4: the roundings of t, exp2f, fp32 sums and
-      // what lies past the bins). Thread t has bins 2 t and 2 t + 1.
+      // and between the whole mass less the rest's most and least weights (1e-4:
+      // the roundings of t, exp2f, fp32 sums). Thread t has bins 2 t, 2 t + 1.
       uint32_t c0 = 0, c1 = 0;
-      if (pass || tid < kNear / 2) {
-        for (int r = 0; r < nrank; ++r) {
-          const uint2 x =
-              *cluster.map_shared_rank(reinterpret_cast<const uint2 *>(sh.fine[sel]) + tid, r);
-          c0 += x.x;
-          c1 += x.y;
-        }
-      }
+      if (pass || tid < window / 2)
+        ranks(reinterpret_cast<uint2 *>(sh.fine[sel]) + tid, [&](int, uint2 v) {
+          c0 += v.x;
+          c1 += v.y;
+        });
       constexpr float kLeast = 0.95760328f;  // 2^(-1/16): a bin's least weight over its most
       const float top = by_mass ? fast_exp2(-0.0625f * (2 * tid - 0.5f) + kWeightBits) : 0.f;
       const float h0 = c0 * top, h1 = c1 * (top * kLeast);
@@ -680,19 +748,26 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
       bool fb0, fb1, fa0, fa1;
       if (by_mass) {
         const float whole = static_cast<float>(total), goal = static_cast<float>(target);
-        const float rest = pass ? hi_all : INFINITY, hi0 = hi_in - h1, slack = 1e-4f * whole;
-        fb0 = fmaxf(hi0 * kLeast, whole - (rest - hi0)) - slack >= goal;
-        fb1 = fmaxf(hi_in * kLeast, whole - (rest - hi_in)) - slack >= goal;
-        fa0 = (pass ? fminf(hi0, whole - (rest - hi0) * kLeast) : hi0) + slack >= goal;
-        fa1 = (pass ? fminf(hi_in, whole - (rest - hi_in) * kLeast) : hi_in) + slack >= goal;
+        const float hi0 = hi_in - h1, slack = 1e-4f * whole;
+        const float seen = whole - (pass ? 0.f : beyond);  // mass of the counted
+        fb0 = fmaxf(hi0 * kLeast, seen - (hi_all - hi0)) - slack >= goal;
+        fb1 = fmaxf(hi_in * kLeast, seen - (hi_all - hi_in)) - slack >= goal;
+        fa0 = fminf(hi0, seen - (hi_all - hi0) * kLeast) + slack >= goal;
+        fa1 = fminf(hi_in, seen - (hi_all - hi_in) * kLeast) + slack >= goal;
       } else {
         fb0 = fa0 = n0 >= static_cast<uint32_t>(top_k);
         fb1 = fa1 = n_in >= static_cast<uint32_t>(top_k);
       }
       // (a bin before the first token's does not count: one token is always kept)
       const int b0 = n0 > 0 ? 2 * tid : 2 * tid + 1;
-      if (n_in > 0 && (fb0 || fb1)) atomicMin(&sh.r_u32[0], fb0 ? b0 : 2 * tid + 1);
-      if (n_in > 0 && (fa0 || fa1)) atomicMin(&sh.r_u32[2], fa0 ? b0 : 2 * tid + 1);
+      const uint32_t wb = __reduce_min_sync(
+          0xffffffffu, n_in > 0 && (fb0 || fb1) ? (fb0 ? b0 : 2 * tid + 1) : kFine);
+      const uint32_t wa = __reduce_min_sync(
+          0xffffffffu, n_in > 0 && (fa0 || fa1) ? (fa0 ? b0 : 2 * tid + 1) : kFine);
+      if (lane == 0) {  // (a warp at a time: an atomic a thread on one word costs microseconds)
+        if (wb < kFine) atomicMin(&sh.r_u32[0], wb);
+        if (wa < kFine) atomicMin(&sh.r_u32[2], wa);
+      }
       __syncthreads();
       fb = static_cast<int>(sh.r_u32[0]), fa = static_cast<int>(sh.r_u32[2]);
       if (tid == fb >> 1) sh.r_u32[1] = fb & 1 ? n_in : n0;
@@ -700,7 +775,7 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
         sh.r_u32[3] = fa == kFine ? n_in : (fa & 1 ? n0 : n0 - c0);
       __syncthreads();
       upto_n = sh.r_u32[1], above_n = sh.r_u32[3];
-      if (fb < kNear) break;
+      if (fb < window) break;
       __syncthreads();
     }
     // fewer than k tokens down to 2^-64: what lies below is never drawn
@@ -712,10 +787,16 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
                              return rw.within(x, fb) && (!cut || thr.takes(x, i));
                            });
       const u64 w = weight_of(c);
-      int rk;
-      u64 before;
-      place_in_list(c, w, &rk, &before);
-      bool keep = c != 0 && (by_mass || rk < top_k);
+      bool keep = c != 0;
+      // a list's 128ths by bin (fb + 1 bins)
+      const uint32_t part =
+          c ? (__float_as_uint(rw.steps(KO::value(comp_key(c))) + kRound) & (kFine - 1)) * 128 /
+                  (fb + 1)
+            : 0;
+      if (!by_mass && static_cast<int>(upto_n) > top_k) {
+        const u64 last = crossing(keep, c, 1, part, 0, top_k);  // (every thread: it has barriers)
+        keep = keep && c >= last;
+      }
       if (use_p) {
         // (mass search: the target is a share of all the row's mass)
         double want = target;
@@ -724,24 +805,19 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
           __syncthreads();
           want = top_p * static_cast<double>(sh.acc[0]);
         }
-        keep = keep && (rk == 0 || static_cast<double>(before) < want);
+        const u64 last = crossing(keep, c, w, part, 0, want);
+        keep = keep && c >= last;
       }
       if (minw > 0.0) keep = keep && rw.scaled(KO::value(comp_key(c))) >= minw;
       accumulate(keep ? w : 0, 1);
-      __syncthreads();  // (also: the list has been read)
-      if (tid < listed) sh.pairs[tid].y = keep ? w : 0;
       __syncthreads();
-      if (keep) {  // mass of the kept tokens with a lower index
-        const u64 at = static_cast<u64>(static_cast<double>(u) * static_cast<double>(sh.acc[1]));
-        const uint32_t low = static_cast<uint32_t>(c) & kIdxMask;
-        u64 cum = 0;
-#pragma unroll 4
-        for (int j = 0; j < listed; ++j) {
-          const ulonglong2 o = sh.pairs[j];
-          if ((static_cast<uint32_t>(o.x) & kIdxMask) > low) cum += o.y;
-        }
-        if (cum <= at && at < cum + w) sh.token = static_cast<int>(comp_idx(c));
-      }
+      // the first token, by index, whose running mass exceeds u's share (weights
+      // are integers: reaches the share's floor and one)
+      const u64 at = static_cast<u64>(static_cast<double>(u) * static_cast<double>(sh.acc[1]));
+      const u64 low = c & kIdxMask;  // falls as the index grows
+      const uint32_t at_part = keep ? comp_idx(c) * 128 / p.vocab : 0;
+      const u64 pick = crossing(keep, low, w, at_part, 0, static_cast<double>(at) + 1.0);
+      if (tid == 0) sh.token = static_cast<int>(kIdxMask - pick);
       __syncthreads();
       done = true;
       break;
@@ -812,7 +888,7 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
       }
       cluster.sync();
       if (by_mass && first) {
-        for (int r = 0; r < nrank; ++r) above_m += *cluster.map_shared_rank(&sh.over, r);
+        ranks(&sh.over, [&](int, u64 v) { above_m += v; });
         above = static_cast<double>(above_m);
       }
       merge(by_mass, target, above, above_m);
@@ -841,16 +917,10 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
         [&](float x) { return x >= least.x; },
         [&](float x, uint32_t i) { return least.takes(x, i) && !most.takes(x, i); });
     const u64 w = by_mass ? weight_of(gc) : (gc ? 1 : 0);
-    int rk;
-    u64 before;
-    place_in_list(gc, w, &rk, &before);
-    before += by_mass ? above_m : static_cast<u64>(above);
-    // the last kept: the first whose running sum reaches the target
-    if (gc && static_cast<double>(before + w) >= target &&
-        (static_cast<double>(before) < target || before == 0))
-      sh.r_u64[3] = gc;
-    __syncthreads();
-    thr = place_of(sh.r_u64[3]);
+    const int shift = max(0, 64 - __clzll(static_cast<long long>(hi - lo)) - 7);
+    const u64 last = crossing(gc != 0, gc, w, gc ? static_cast<uint32_t>((hi - gc) >> shift) : 0,
+                              by_mass ? above_m : static_cast<u64>(above), target);
+    if (last) thr = place_of(last);
     cut = true;
     __syncthreads();
   }
@@ -860,7 +930,7 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
     p.out[row] = token;
     if (p.logprob) {
       double s = 0;
-      for (int r = 0; r < nrank; ++r) s += *cluster.map_shared_rank(&sh.lsum, r);
+      ranks(&sh.lsum, [&](int, double v) { s += v; });
       const double d = x == rw.fmax_ ? 0.0 : static_cast<double>(x) - rw.xmax;
       p.logprob[row] = static_cast<float>(d - log(s));
     }
@@ -881,8 +951,7 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
     if (lane == 0) atomicMin(&sh.first, first);
     cluster.sync();  // (every CTA's lsum is written, too)
     if (rank == 0 && tid == 0) {
-      for (int r = 0; r < nrank; ++r)
-        first = min(first, *cluster.map_shared_rank(&sh.first, r));
+      ranks(&sh.first, [&](int, uint32_t v) { first = min(first, v); });
       finish(rw.fmax_, static_cast<int>(first));
     }
   } else if (done) {
@@ -936,12 +1005,11 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
     }
     cluster.sync();
     u64 total = 0, before = 0, own = 0;
-    for (int r = 0; r < nrank; ++r) {
-      const u64 x = *cluster.map_shared_rank(&sh.mass, r);
+    ranks(&sh.mass, [&](int r, u64 x) {
       if (r < rank) before += x;
       if (r == rank) own = x;
       total += x;
-    }
+    });
     const u64 at = static_cast<u64>(static_cast<double>(u) * static_cast<double>(total));
     if (at >= before && at < before + own) {
       u64 wb = before;
@@ -992,15 +1060,16 @@ template <typename T>
 int launch_sample(SampleParams p, cudaStream_t s) {
   using K = typename KeyOf<T>::K;
   static std::atomic<unsigned long long> attr_set{0};
-  constexpr int kSmemMax = 227 * 1024;
+  constexpr int kSmemMax = 227 * 1024, kSmemTwo = 112 * 1024;
   if (smem_limit_once(attr_set, sample_kernel<T>, kSmemMax) != cudaSuccess)
     return check_launch("sample_kernel smem attribute");
   const size_t fixed = (sizeof(Shared) + 15) / 16 * 16 + 64;
-  // CTAs per row: at least what the row needs of shared memory; more while
-  // that adds CTAs up to two per SM and leaves 4096 tokens to each
+  // CTAs per row: as many as bring the shared memory down to two CTAs per SM
+  // (one CTA's barriers pass under the other's work); more while that adds CTAs
+  // up to two per SM and leaves 2048 tokens to each
   auto slice_of = [&](int c) { return ((p.vocab + c - 1) / c + 7) / 8 * 8; };
   int c = 1;
-  while (c < kMaxCluster && fixed + size_t(slice_of(c)) * sizeof(K) > size_t(kSmemMax)) c *= 2;
+  while (c < kMaxCluster && fixed + size_t(slice_of(c)) * sizeof(K) > size_t(kSmemTwo)) c *= 2;
   while (c < kMaxCluster && int64_t(p.rows) * c * 2 <= 2 * num_sms() && slice_of(2 * c) >= 2048)
     c *= 2;
   p.slice = slice_of(c);
