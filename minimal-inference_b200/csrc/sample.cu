@@ -226,7 +226,6 @@ struct Shared {
     ulonglong2 pairs[kCap];         // entries of the gathered list: order, weight
   };
   u64 list[kCap];   // this CTA's gathered composites
-  float2 queue[kSWarps][64];        // per warp: tokens waiting for their weight
   u64 share[128];                   // a long list's sums per 128th
   u64 acc[4];                       // integer sums over the list; [3]: entries in pairs
   u64 cross;
@@ -395,23 +394,31 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
   rw.fscale = static_cast<float>(fmin(fmax(16.0 * rw.c, 1e-30), 3e38));
   rw.table = sh.table;
 
-  // Visits this thread's tokens above -inf (vectors of its warp in order):
-  // f(bits, logit, token). A vector whose largest logit pre() turns down is
-  // passed over: one test for VEC tokens, most of which no search is after.
-  auto each = [&](auto &&pre, auto &&f) {
+  // f(logit, token) for this thread's tokens above -inf that in(logit, token)
+  // accepts, none of them below least_x: one test passes over a vector of VEC
+  // tokens, as most are. The tests run over the whole vector, f over a mask of
+  // what they found: f's code once (it may be long), and as often as a lane of
+  // the warp needs it.
+  auto each = [&](float least_x, auto &&in, auto &&f) {
     for (int v = v0 + lane; v < v1; v += 32) {
       const uint4 raw = *reinterpret_cast<const uint4 *>(keys + v * VEC);
-      if (!pre(KO::max_of(vec_top(raw)))) continue;
+      if (!(KO::max_of(vec_top(raw)) >= least_x)) continue;
       const K *e = reinterpret_cast<const K *>(&raw);
       const int i0 = base + v * VEC - pad;
+      uint32_t found = 0;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const float x = KO::raw(e[j]);
-        if (x > -INFINITY) f(e[j], x, static_cast<uint32_t>(i0 + j));
+        if (x > -INFINITY && in(x, static_cast<uint32_t>(i0 + j))) found |= 1u << j;
+      }
+      while (found) {
+        const int j = __ffs(found) - 1;
+        found &= found - 1;
+        f(KO::raw(keys[v * VEC + j]), static_cast<uint32_t>(i0 + j));
       }
     }
   };
-  auto comp_of = [&](K bits, uint32_t i) { return composite(KO::key(bits), i); };
+  auto comp_of = [&](float x, uint32_t i) { return composite(KO::key(KO::bits(x)), i); };
   // one value per thread summed over the CTA in a fixed order; thread 0 has it
   auto block_sum = [&](double d, double *part) {
 #pragma unroll
@@ -487,13 +494,11 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
   };
   // Gathers the tokens f accepts (at most kCap over the cluster), sorts them:
   // this thread's composite in descending order (0: none).
-  auto gather = [&](auto &&pre, auto &&f) {
+  auto gather = [&](float least_x, auto &&in) {
     uint32_t *cnt = &sh.list_n[sel & 1];
-    each(pre, [&](K bits, float x, uint32_t i) {
-      if (f(x, i)) {
-        const uint32_t at = atomicAdd(cnt, 1u);
-        if (at < kCap) sh.list[at] = comp_of(bits, i);
-      }
+    each(least_x, in, [&](float x, uint32_t i) {
+      const uint32_t at = atomicAdd(cnt, 1u);
+      if (at < kCap) sh.list[at] = comp_of(x, i);
     });
     cluster.sync();
     // this thread's entry of the ranks' lists, one after the other
@@ -575,41 +580,6 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (lane == 0 && v) atomicAdd(&sh.acc[slot], v);
   };
-  // Calls f(logit, token) for the tokens in(logit, token) accepts, whole warps at
-  // a time: few tokens of a row are, and a weight is some 40 instructions.
-  auto packed = [&](float least_x, auto &&in, auto &&f) {
-    float2 *q = sh.queue[warp];
-    int have = 0;
-    for (int vw = v0; vw < v1; vw += 32) {
-      uint4 raw = make_uint4(empty, empty, empty, empty);
-      if (vw + lane < v1) raw = *reinterpret_cast<const uint4 *>(keys + (vw + lane) * VEC);
-      const K *e = reinterpret_cast<const K *>(&raw);
-      const int i0 = base + (vw + lane) * VEC - pad;
-      if (!__any_sync(0xffffffffu, KO::max_of(vec_top(raw)) >= least_x)) continue;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float x = KO::raw(e[j]);
-        const bool mine = x > -INFINITY && in(x, static_cast<uint32_t>(i0 + j));
-        const uint32_t m = __ballot_sync(0xffffffffu, mine);
-        if (m == 0) continue;
-        if (mine)
-          q[have + __popc(m & ((1u << lane) - 1u))] = make_float2(x, __int_as_float(i0 + j));
-        have += __popc(m);
-        __syncwarp();
-        if (have >= 32) {
-          const float2 t = q[lane], rest = q[32 + lane];
-          __syncwarp();
-          have -= 32;
-          if (lane < have) q[lane] = rest;
-          __syncwarp();
-          f(t.x, __float_as_uint(t.y));
-        }
-      }
-    }
-    if (lane < have) f(q[lane].x, __float_as_uint(q[lane].y));
-    __syncwarp();
-  };
-
   // ordered key of the largest logit (its float maps back to the type's bits)
   auto key_of_max = [&]() -> uint32_t { return KO::key(KO::bits(rw.fmax_)); };
   // ---- 2. to 4. the filters' thresholds ----------------------------------------
@@ -782,10 +752,11 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
     if (!by_mass && fb == kFine) continue;
     if (fb < kFine && upto_n <= kCap) {
       // -- 3. everything that may be kept fits the list
-      const u64 c = gather([&](float x) { return rw.within(x, fb); },
-                           [&](float x, uint32_t i) {
-                             return rw.within(x, fb) && (!cut || thr.takes(x, i));
-                           });
+      // (half a bin below what bin fb takes: more than the roundings)
+      const float least_x = rw.fmax_ - (fb + 1.f) / rw.fscale;
+      const u64 c = gather(least_x, [&](float x, uint32_t i) {
+        return rw.within(x, fb) && (!cut || thr.takes(x, i));
+      });
       const u64 w = weight_of(c);
       bool keep = c != 0;
       // a list's 128ths by bin (fb + 1 bins)
@@ -864,7 +835,7 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
       u64 over = 0;
       const bool first = inside == UINT32_MAX;
       const Place least = place_of(lo), most = place_of(hi + 1);  // range: takes least, not most
-      packed(
+      each(
           least.x,
           [&](float x, uint32_t i) {
             return least.takes(x, i) && ((by_mass && first) || !most.takes(x, i));
@@ -874,7 +845,7 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
             if (most.takes(x, i))
               over += w;
             else
-              add(static_cast<int>((hi - comp_of(KO::bits(x), i)) >> shift), by_mass, w);
+              add(static_cast<int>((hi - comp_of(x, i)) >> shift), by_mass, w);
           });
       if (by_mass && first) {
 #pragma unroll
@@ -914,8 +885,7 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
     }
     const Place least = place_of(lo), most = place_of(hi + 1);
     const u64 gc = gather(
-        [&](float x) { return x >= least.x; },
-        [&](float x, uint32_t i) { return least.takes(x, i) && !most.takes(x, i); });
+        least.x, [&](float x, uint32_t i) { return least.takes(x, i) && !most.takes(x, i); });
     const u64 w = by_mass ? weight_of(gc) : (gc ? 1 : 0);
     const int shift = max(0, 64 - __clzll(static_cast<long long>(hi - lo)) - 7);
     const u64 last = crossing(gc != 0, gc, w, gc ? static_cast<uint32_t>((hi - gc) >> shift) : 0,
@@ -943,10 +913,9 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
     }
   } else if (greedy) {
     uint32_t first = 0xFFFFFFFFu;
-    each([&](float x) { return x == rw.fmax_; },
-         [&](K, float x, uint32_t i) {
-           if (x == rw.fmax_) first = min(first, i);
-         });
+    each(
+        rw.fmax_, [&](float x, uint32_t) { return x == rw.fmax_; },
+        [&](float, uint32_t i) { first = min(first, i); });
     first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) atomicMin(&sh.first, first);
     cluster.sync();  // (every CTA's lsum is written, too)
@@ -978,12 +947,13 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
     };
     u64 m = 0;
     if (cut) {
-      packed(thr.x, [&](float x, uint32_t i) { return thr.takes(x, i); },
-             [&](float x, uint32_t) {
-               const double d = rw.scaled(x);
-               m += d >= minw ? RowW::whole(d) : 0ull;
-             });
-    } else {  // all tokens: no need to pack
+      each(
+          thr.x, [&](float x, uint32_t i) { return thr.takes(x, i); },
+          [&](float x, uint32_t) {
+            const double d = rw.scaled(x);
+            m += d >= minw ? RowW::whole(d) : 0ull;
+          });
+    } else {  // all tokens: whole vectors
       for (int vw = v0; vw < v1; vw += 32) {
         uint4 raw = make_uint4(empty, empty, empty, empty);
         if (vw + lane < v1) raw = *reinterpret_cast<const uint4 *>(keys + (vw + lane) * VEC);
