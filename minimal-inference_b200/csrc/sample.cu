@@ -629,14 +629,24 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
         }
         sum += part;
       }
-      if (near) {
+      if (near && by_mass) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const float z = t[j] + kRound;
           if (z <= kRound + (window - 1)) {
             count(z);
-            if (by_mass) inside += w[j];
+            inside += w[j];
           }
+        }
+      } else if (near) {  // few: a mask, then a loop over what it found
+        uint32_t found = 0;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (t[j] + kRound <= kRound + (window - 1)) found |= 1u << j;
+        while (found) {
+          const int j = __ffs(found) - 1;
+          found &= found - 1;
+          count(rw.steps(KO::raw(keys[v * VEC + j])) + kRound);
         }
       }
     }
