@@ -13,11 +13,14 @@
 // every page_size steps thus moves about a page and the recent window per
 // head instead of the whole cache.
 //
-// One CTA per (layer, request, head): the threshold score by radix select (8
-// bits a pass) over the ordered bits; a bit per token in shared memory with
-// running counts per 32-bit word, from which the i-th hole and the i-th token
-// to move are found by bisection; then one warp per row pair (K and V), 16
-// bytes a lane. HBM traffic is the scores once and the moved rows twice.
+// One CTA per (layer, request, head). The scores are read once, as ordered bits
+// in shared memory (requests past kKeyCap tokens read them again each pass).
+// The threshold is found by radix select, 11 bits a pass: the first digit then
+// has two bits of mantissa, and a few hundred scores of like size do not all
+// meet in one counter. A bit per token in shared memory with running counts
+// per 32-bit word gives the i-th hole and the i-th token to move by bisection.
+// Rows move a pair (K and V) per warp step, 16 bytes a lane, kRows pairs loaded
+// before any is stored. HBM traffic is the scores once and the moved rows twice.
 #include <algorithm>
 
 #include "mi_common.cuh"
@@ -27,7 +30,9 @@ namespace {
 
 constexpr int kEThreads = 256;
 constexpr int kEWarps = kEThreads / 32;
-constexpr int kShiftRows = 8;  // rows a warp holds while the recent window moves
+constexpr int kRows = 8;       // row pairs a warp holds in registers while they move
+constexpr int kDigit = 11;     // radix select: 11, 11 and 10 bits
+constexpr int kKeyCap = 8192;  // tokens whose ordered scores are kept in shared memory
 constexpr int kESmemMax = 200 * 1024;
 
 struct EvictParams {
@@ -39,7 +44,7 @@ struct EvictParams {
   int64_t num_pages;
   int ps, hkv, row_bytes;  // row: one head of one token of K (or V)
   const int32_t *indptr, *indices, *last;
-  int batch, budget, recent, sinks, max_len;
+  int batch, budget, recent, sinks, max_len, key_cap;
   int32_t *kept;
   int32_t *status;
 };
@@ -52,14 +57,34 @@ __device__ __forceinline__ uint32_t score_key(float x) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// VB: bytes a lane copies at once (16 where rows and pointers allow).
+// Position of the n-th (from 0) set bit of w, which has more than n.
+__device__ __forceinline__ int nth_bit(uint32_t w, int n) {
+  int at = 0;
+#pragma unroll
+  for (int half = 16; half > 0; half >>= 1) {
+    const int c = __popc((w >> at) & ((1u << half) - 1u));
+    if (n >= c) {
+      n -= c;
+      at += half;
+    }
+  }
+  return at;
+}
+
+struct RowPair {
+  const unsigned char *src;  // K rows of two slots
+  unsigned char *dst;
+};
+
+// V: what a lane copies at once (16 bytes where rows and pointers allow).
 template <typename V>
 __global__ void __launch_bounds__(kEThreads) evict_kernel(const EvictParams p) {
   extern __shared__ uint32_t s_dyn[];
-  __shared__ uint32_t s_hist[256];
+  __shared__ uint32_t s_hist[1 << kDigit];
   __shared__ int s_warp[kEWarps];
-  __shared__ uint32_t s_digit, s_need;
+  __shared__ uint32_t s_digit, s_need, s_in;
   __shared__ int s_bad;
+  __shared__ RowPair s_pair[kEWarps][32];
   const int b = blockIdx.x / p.hkv, h = blockIdx.x % p.hkv, layer = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n = kv_len_of(p.indptr, p.last, b, p.ps);
@@ -92,80 +117,98 @@ __global__ void __launch_bounds__(kEThreads) evict_kernel(const EvictParams p) {
   const int low = p.budget - recent, mid_end = n - recent;
   const int want = low - sinks;  // of the middle tokens [sinks, mid_end)
 
-  // ---- threshold: key of the want-th largest score, and how many ties to keep
-  uint32_t prefix = 0, need = want;
-  if (want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kEThreads) s_hist[i] = 0;
-      __syncthreads();
-      for (int t = sinks + tid; t < mid_end; t += kEThreads) {
-        const uint32_t k = score_key(*score_at(t));
-        if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&s_hist[(k >> shift) & 255], 1u);
-      }
-      __syncthreads();
-      if (warp == 0) {  // from the largest digit down: 8 per lane
-        uint32_t c[8], sum = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum += c[i] = s_hist[255 - (lane * 8 + i)];
-        uint32_t incl = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += y;
-        }
-        uint32_t before = incl - sum;
-        if (before < need && need <= incl) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            if (before < need && need <= before + c[i]) {
-              s_digit = 255 - (lane * 8 + i);
-              s_need = need - before;
-            }
-            before += c[i];
-          }
-        }
-      }
-      __syncthreads();
-      prefix = (prefix << 8) | s_digit;
-      need = s_need;  // of the tokens with this prefix
-    }
-  }
-  // ---- a bit per token: kept --------------------------------------------------
   const int words = (n + 31) / 32;
   uint32_t *bits = s_dyn, *before = s_dyn + words;  // kept tokens in earlier words
+  uint32_t *keys = s_dyn + (p.max_len + 31) / 32 * 2;
+  const bool held = n <= p.key_cap;
+  auto key_of = [&](int t) { return held ? keys[t] : score_key(*score_at(t)); };
+  if (held && want > 0) {
+    for (int t = sinks + tid; t < mid_end; t += kEThreads) keys[t] = score_key(*score_at(t));
+  }
+  // ---- threshold: key of the want-th largest score, and how many ties to keep
+  // (need < in: of `in` tokens with that key; else all with key >= cut are kept)
+  uint32_t cut = 0, need = want, in = 0;
+  int left = 32;  // bits not looked at yet
+  while (want > 0 && left > 0 && need != in) {
+    const int width = min(kDigit, left), shift = left - width;
+    for (int i = tid; i < (1 << kDigit); i += kEThreads) s_hist[i] = 0;
+    __syncthreads();
+    for (int t = sinks + tid; t < mid_end; t += kEThreads) {
+      const uint32_t k = key_of(t);
+      if (left == 32 || (k >> left) == (cut >> left))
+        atomicAdd(&s_hist[(k >> shift) & ((1u << width) - 1u)], 1u);
+    }
+    __syncthreads();
+    // from the largest digit down, 8 a thread
+    constexpr int kPer = (1 << kDigit) / kEThreads;
+    const int top = (1 << kDigit) - 1 - tid * kPer;
+    uint32_t c[kPer], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sum += c[i] = s_hist[top - i];
+    uint32_t incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) s_warp[warp] = incl;
+    __syncthreads();
+    for (int i = 0; i < warp; ++i) incl += s_warp[i];
+    uint32_t first = incl - sum;
+    if (first < need && need <= incl) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        if (first < need && need <= first + c[i]) {
+          s_digit = top - i;
+          s_need = need - first;
+          s_in = c[i];
+        }
+        first += c[i];
+      }
+    }
+    __syncthreads();
+    cut |= s_digit << shift;
+    need = s_need;
+    in = s_in;
+    left = shift;
+    __syncthreads();
+  }
+  // ---- a bit per token: kept --------------------------------------------------
   const int per_warp = (words + kEWarps - 1) / kEWarps;
   const int w0 = min(words, warp * per_warp), w1 = min(words, w0 + per_warp);
-  auto key_of = [&](int t) {  // 0 outside the middle and for NaN; ordered keys are > 0
-    return (t >= sinks && t < mid_end) ? score_key(*score_at(t)) : 0u;
-  };
-  // ties with the threshold, per warp segment, so each segment knows its first's rank
-  int ties = 0;
-  for (int w = w0; w < w1; ++w) {
-    const int t = w * 32 + lane;
-    const bool tie = want > 0 && t >= sinks && t < mid_end && key_of(t) == prefix;
-    ties += __popc(__ballot_sync(0xffffffffu, tie));
-  }
-  if (lane == 0) s_warp[warp] = ties;
-  __syncthreads();
+  // ties with the threshold, where some are left out: their number per warp
+  // segment, so that each segment knows its first's rank
   uint32_t rank = 0;
-  for (int i = 0; i < warp; ++i) rank += s_warp[i];
-  __syncthreads();
+  const bool some = want > 0 && need < in;
+  if (some) {
+    int ties = 0;
+    for (int w = w0; w < w1; ++w) {
+      const int t = w * 32 + lane;
+      const bool tie = t >= sinks && t < mid_end && key_of(t) == cut;
+      ties += __popc(__ballot_sync(0xffffffffu, tie));
+    }
+    if (lane == 0) s_warp[warp] = ties;
+    __syncthreads();
+    for (int i = 0; i < warp; ++i) rank += s_warp[i];
+    __syncthreads();
+  }
   int count = 0;
   for (int w = w0; w < w1; ++w) {
     const int t = w * 32 + lane;
     const bool mid = t >= sinks && t < mid_end;
-    const uint32_t k = key_of(t);
-    const bool tie = want > 0 && mid && k == prefix;
-    const uint32_t tm = __ballot_sync(0xffffffffu, tie);
-    const bool keep =
-        t < n && (!mid || (want > 0 && (k > prefix ||
-                                        (tie && rank + __popc(tm & ((1u << lane) - 1u)) < need))));
+    const uint32_t k = mid && want > 0 ? key_of(t) : 0;
+    bool keep = mid ? want > 0 && k >= cut : t < n;
+    if (some) {
+      const bool tie = mid && k == cut;
+      const uint32_t tm = __ballot_sync(0xffffffffu, tie);
+      if (tie) keep = rank + __popc(tm & ((1u << lane) - 1u)) < need;
+      rank += __popc(tm);
+    }
     const uint32_t m = __ballot_sync(0xffffffffu, keep);
     if (lane == 0) {
       bits[w] = m;
       before[w] = count;
     }
-    rank += __popc(tm);
     count += __popc(m);
   }
   if (lane == 0) s_warp[warp] = count;
@@ -204,27 +247,35 @@ __global__ void __launch_bounds__(kEThreads) evict_kernel(const EvictParams p) {
         const int m = (l + r + 1) >> 1;
         if (m * 32 - static_cast<int>(before[m]) <= i) l = m; else r = m - 1;
       }
-      dst = l * 32 + __fns(~bits[l], 0, i - (l * 32 - static_cast<int>(before[l])) + 1);
+      dst = l * 32 + nth_bit(~bits[l], i - (l * 32 - static_cast<int>(before[l])));
       const int q = kept_before(low) + i;  // the q-th kept token overall
       l = 0, r = words - 1;
       while (l < r) {
         const int m = (l + r + 1) >> 1;
         if (static_cast<int>(before[m]) <= q) l = m; else r = m - 1;
       }
-      src = l * 32 + __fns(bits[l], 0, q - static_cast<int>(before[l]) + 1);
+      src = l * 32 + nth_bit(bits[l], q - static_cast<int>(before[l]));
       *score_at(dst) = *score_at(src);
       if (kept) kept[dst] = src;
+      s_pair[warp][lane] = RowPair{k_row(src), k_row(dst)};
     }
+    __syncwarp();
     const int cnt = min(32, moves - i0);
-    for (int j = 0; j < cnt; ++j) {
-      const int d = __shfl_sync(0xffffffffu, dst, j), s = __shfl_sync(0xffffffffu, src, j);
-      unsigned char *dp = k_row(d), *sp = k_row(s);
+    for (int j = 0; j < cnt; j += kRows) {
       for (int e = lane; e < 2 * vec; e += 32) {
         const int64_t off = (e < vec ? 0 : v_off) +
                             static_cast<int64_t>(e < vec ? e : e - vec) * sizeof(V);
-        *reinterpret_cast<V *>(dp + off) = *reinterpret_cast<const V *>(sp + off);
+        V hold[kRows];
+        // (row addresses come from each lane's own pair)
+#pragma unroll
+        for (int u = 0; u < kRows; ++u)
+          if (j + u < cnt) hold[u] = *reinterpret_cast<const V *>(s_pair[warp][j + u].src + off);
+#pragma unroll
+        for (int u = 0; u < kRows; ++u)
+          if (j + u < cnt) *reinterpret_cast<V *>(s_pair[warp][j + u].dst + off) = hold[u];
       }
     }
+    __syncwarp();
   }
   if (kept)
     for (int j = tid; j < low; j += kEThreads)
@@ -232,23 +283,23 @@ __global__ void __launch_bounds__(kEThreads) evict_kernel(const EvictParams p) {
   // ---- the recent window moves down by n - budget, lowest first ---------------
   // (the rows above may be read from where the window goes)
   const int by = n - p.budget;
-  constexpr int kChunk = kEWarps * kShiftRows;
+  constexpr int kChunk = kEWarps * kRows;
   for (int c0 = 0; c0 < recent; c0 += kChunk) {
     __syncthreads();
     for (int e0 = 0; e0 < 2 * vec; e0 += 32) {  // a row pair wider than a warp: in parts
       const int e = e0 + lane;
       const int64_t off = (e < vec ? 0 : v_off) +
                           static_cast<int64_t>(e < vec ? e : e - vec) * sizeof(V);
-      V hold[kShiftRows];
+      V hold[kRows];
 #pragma unroll
-      for (int j = 0; j < kShiftRows; ++j) {
+      for (int j = 0; j < kRows; ++j) {
         const int r = c0 + j * kEWarps + warp;
         if (r < recent && e < 2 * vec)
           hold[j] = *reinterpret_cast<const V *>(k_row(low + r + by) + off);
       }
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < kShiftRows; ++j) {
+      for (int j = 0; j < kRows; ++j) {
         const int r = c0 + j * kEWarps + warp;
         if (r < recent && e < 2 * vec) *reinterpret_cast<V *>(k_row(low + r) + off) = hold[j];
       }
@@ -312,8 +363,10 @@ extern "C" int mi_kv_evict(void *const *layer_pools, void *kv_data, int64_t kv_l
   EvictParams p{layer_pools, static_cast<unsigned char *>(kv_data), kv_layer_stride * es, scores,
                 num_pages * num_kv_heads * page_size, num_pages, page_size, num_kv_heads,
                 static_cast<int>(row), kv_indptr, kv_indices, kv_last_page_len, batch_size, budget,
-                recent, sinks, static_cast<int>(std::min<int64_t>(max_len, cap)), kept, status};
-  const int smem = (p.max_len + 31) / 32 * 8;
+                recent, sinks, static_cast<int>(std::min<int64_t>(max_len, cap)), 0, kept, status};
+  const int map = (p.max_len + 31) / 32 * 8;
+  p.key_cap = std::min({p.max_len, kKeyCap, (kESmemMax - map) / 4});
+  const int smem = map + p.key_cap * 4;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   // torch's pools are 256-byte aligned; a caller's own need only be aligned to
   // the element, and then the copies are narrower. (With layer_pools the
