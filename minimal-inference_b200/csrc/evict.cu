@@ -32,7 +32,7 @@ constexpr int kEThreads = 256;
 constexpr int kEWarps = kEThreads / 32;
 constexpr int kRows = 8;       // row pairs a warp holds in registers while they move
 constexpr int kDigit = 11;     // radix select: 11, 11 and 10 bits
-constexpr int kKeyCap = 8192;  // tokens whose ordered scores are kept in shared memory
+constexpr int kKeyCap = 4096;  // tokens whose ordered scores are kept in shared memory
 constexpr int kESmemMax = 200 * 1024;
 
 struct EvictParams {
@@ -78,7 +78,8 @@ struct RowPair {
 
 // V: what a lane copies at once (16 bytes where rows and pointers allow).
 template <typename V>
-__global__ void __launch_bounds__(kEThreads) evict_kernel(const EvictParams p) {
+// four CTAs per SM (64 registers): most of a CTA's time is latency
+__global__ void __launch_bounds__(kEThreads, 4) evict_kernel(const EvictParams p) {
   extern __shared__ uint32_t s_dyn[];
   __shared__ uint32_t s_hist[1 << kDigit];
   __shared__ int s_warp[kEWarps];
@@ -116,6 +117,16 @@ __global__ void __launch_bounds__(kEThreads) evict_kernel(const EvictParams p) {
   const int recent = min(p.recent, p.budget), sinks = min(p.sinks, p.budget - recent);
   const int low = p.budget - recent, mid_end = n - recent;
   const int want = low - sinks;  // of the middle tokens [sinks, mid_end)
+
+  unsigned char *kv = p.layer_kv ? static_cast<unsigned char *>(p.layer_kv[layer])
+                                 : p.kv + layer * p.kv_stride;
+  const int64_t slot_bytes = static_cast<int64_t>(p.hkv) * p.row_bytes;
+  auto k_row = [&](int t) -> unsigned char * {
+    return kv + (static_cast<int64_t>(table[t / p.ps]) * 2 * p.ps + t % p.ps) * slot_bytes +
+           static_cast<int64_t>(h) * p.row_bytes;
+  };
+  const int64_t v_off = p.ps * slot_bytes;  // from a K row to its V row
+  const int vec = p.row_bytes / static_cast<int>(sizeof(V));  // vectors of a row
 
   const int words = (n + 31) / 32;
   uint32_t *bits = s_dyn, *before = s_dyn + words;  // kept tokens in earlier words
@@ -226,16 +237,6 @@ __global__ void __launch_bounds__(kEThreads) evict_kernel(const EvictParams p) {
   };
   const int moves = want - (kept_before(low) - sinks);  // holes below low = tokens to move there
 
-  unsigned char *kv = p.layer_kv ? static_cast<unsigned char *>(p.layer_kv[layer])
-                                 : p.kv + layer * p.kv_stride;
-  const int64_t slot_bytes = static_cast<int64_t>(p.hkv) * p.row_bytes;
-  auto k_row = [&](int t) -> unsigned char * {
-    return kv + (static_cast<int64_t>(table[t / p.ps]) * 2 * p.ps + t % p.ps) * slot_bytes +
-           static_cast<int64_t>(h) * p.row_bytes;
-  };
-  const int64_t v_off = p.ps * slot_bytes;  // from a K row to its V row
-  const int vec = p.row_bytes / static_cast<int>(sizeof(V));  // vectors of a row
-
   // ---- holes: the i-th takes the i-th kept token at or past `low` -------------
   for (int i0 = warp * 32; i0 < moves; i0 += kEWarps * 32) {
     const int i = i0 + lane;
@@ -281,35 +282,51 @@ __global__ void __launch_bounds__(kEThreads) evict_kernel(const EvictParams p) {
     for (int j = tid; j < low; j += kEThreads)
       if ((bits[j >> 5] >> (j & 31)) & 1u) kept[j] = j;
   // ---- the recent window moves down by n - budget, lowest first ---------------
-  // (the rows above may be read from where the window goes)
+  // A slot may be written once it has been read, as the source of an earlier
+  // one (or of a row above): rows go in chunks, a barrier between a chunk's
+  // loads and its stores; the next chunk's loads follow its stores at once.
   const int by = n - p.budget;
   constexpr int kChunk = kEWarps * kRows;
-  for (int c0 = 0; c0 < recent; c0 += kChunk) {
-    __syncthreads();
+  for (int c0 = 0; c0 < recent; c0 += kEWarps * 32) {
+    {
+      const int r = c0 + lane * kEWarps + warp;
+      if (r < recent) s_pair[warp][lane] = RowPair{k_row(low + r + by), k_row(low + r)};
+    }
+    __syncwarp();
+    // rows of this warp in this block of 256
+    const int mine = max(0, min(32, (recent - c0 - warp + kEWarps - 1) / kEWarps));
+    const int chunks = (min(recent - c0, kEWarps * 32) + kChunk - 1) / kChunk;
     for (int e0 = 0; e0 < 2 * vec; e0 += 32) {  // a row pair wider than a warp: in parts
       const int e = e0 + lane;
+      const bool on = e < 2 * vec;
       const int64_t off = (e < vec ? 0 : v_off) +
                           static_cast<int64_t>(e < vec ? e : e - vec) * sizeof(V);
       V hold[kRows];
+      auto load = [&](int c) {
 #pragma unroll
-      for (int j = 0; j < kRows; ++j) {
-        const int r = c0 + j * kEWarps + warp;
-        if (r < recent && e < 2 * vec)
-          hold[j] = *reinterpret_cast<const V *>(k_row(low + r + by) + off);
-      }
-      __syncthreads();
+        for (int u = 0; u < kRows; ++u)
+          if (on && c * kRows + u < mine)
+            hold[u] = *reinterpret_cast<const V *>(s_pair[warp][c * kRows + u].src + off);
+      };
+      __syncthreads();  // (moves above, or the part or block before, have read)
+      load(0);
+      for (int c = 0; c < chunks; ++c) {
+        __syncthreads();
 #pragma unroll
-      for (int j = 0; j < kRows; ++j) {
-        const int r = c0 + j * kEWarps + warp;
-        if (r < recent && e < 2 * vec) *reinterpret_cast<V *>(k_row(low + r) + off) = hold[j];
+        for (int u = 0; u < kRows; ++u)
+          if (on && c * kRows + u < mine)
+            *reinterpret_cast<V *>(s_pair[warp][c * kRows + u].dst + off) = hold[u];
+        if (c + 1 < chunks) load(c + 1);
       }
     }
+    __syncwarp();
+  }
+  for (int c0 = 0; c0 < recent; c0 += kEThreads) {
     const int r = c0 + tid;
-    const bool mine = tid < kChunk && r < recent;
     float sv = 0.f;
-    if (mine) sv = *score_at(low + r + by);
+    if (r < recent) sv = *score_at(low + r + by);
     __syncthreads();
-    if (mine) {
+    if (r < recent) {
       *score_at(low + r) = sv;
       if (kept) kept[low + r] = low + r + by;
     }
