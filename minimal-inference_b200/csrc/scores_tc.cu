@@ -7,21 +7,23 @@
 // rows the columns, so a thread owns one key and the sum over queries stays in
 // its registers (rows on the lanes would need a reduction across threads for
 // every column). Per element that leaves a scale-and-subtract of the row's
-// log-sum-exp, an exp2 and an addition: the exp2 unit (16 per clock and SM)
-// bounds the kernel at 1024 clocks a tile, four times the tensor core's 256.
+// log-sum-exp, an exp2 and an addition. The exp2 unit (16 per clock and SM)
+// takes 1024 clocks a tile; shared memory, which bounds the kernel, takes 512
+// for the operands of the 128 x 128 x 128 product, 512 for the row terms (a
+// clock per 32 lanes and column) and 256 for the Q tile's arrival. Measured
+// (16 prompts of 100-1500 tokens, 32/8 heads of 128): 96 us, 1.7 times that
+// bound of 1280 clocks a tile. Tried without gain: quarters or halves of a
+// tile to a group, four groups, 256 keys to an item, K tiles an item ahead.
 //
-// Persistent, one CTA per SM, items from a counter in the workspace, those with
-// the most queries first (of all requests: an item may be half of an SM's share
-// of the work, and taken late it would leave the others waiting). 18 warps:
+// Persistent, one CTA per SM, items from a counter in the workspace, a
+// request's first keys (most queries) first. 10 warps:
 //   warp 0     producer: TMA loads of the K tile (16-token boxes straight from
 //              the pages) and the Q tiles, two K and three Q stages;
 //   warp 1     MMA issuer, four 128-column TMEM accumulators;
-//   warps 2-17 four groups of four, each with a quarter of every tile's columns:
-//              lane = key. (Groups that took whole tiles in turn had an
-//              accumulator each, and waited for its next product.)
-// Each warp keeps its 32 columns' row terms in a shared-memory slice of its own
-// (read as broadcasts), loaded one tile ahead. The other groups hand their sums
-// to the first at the end of an item: a key's sum has a fixed order.
+//   warps 2-9  two groups of four take the tiles in turn: lane = key.
+// Each warp keeps the tile's 128 row terms in a shared-memory slice of its own
+// (read as broadcasts), loaded one tile ahead. The second group hands its sums
+// to the first at the end of an item, so a key's sum has a fixed order.
 // Every wait is bounded; TMEM is freed on every path.
 #include <algorithm>
 #include <type_traits>
@@ -35,10 +37,9 @@ namespace {
 
 constexpr int kKeys = 128;      // keys per item (TMEM lanes)
 constexpr int kRows = 128;      // packed query rows per tile (columns)
-constexpr int kGroups = 4;      // summing groups of four warps
-constexpr int kCols = kRows / kGroups;
-constexpr int kScThreads = 64 + kGroups * 128;
+constexpr int kScThreads = 320;
 constexpr int kScMaxBatch = 1024;
+constexpr int kScSortBatch = 128;
 constexpr int kQStages = 3, kKStages = 2, kAcc = 4, kRecs = 4;
 
 template <int D> struct ScLayout {
@@ -47,12 +48,12 @@ template <int D> struct ScLayout {
   static constexpr int K_BYTES = DH * kKeys * 128;
   static constexpr int K_OFF = 0;
   static constexpr int Q_OFF = kKStages * K_BYTES;
-  static constexpr int LSE_OFF = Q_OFF + kQStages * Q_BYTES;  // [warp][2][32] fp32
-  static constexpr int PART_OFF = LSE_OFF + 4 * kGroups * 2 * kCols * 4;  // [group - 1][128] fp32
-  static constexpr int REC_OFF = PART_OFF + (kGroups - 1) * kKeys * 4;
+  static constexpr int LSE_OFF = Q_OFF + kQStages * Q_BYTES;  // [8 warps][2][128] fp32
+  static constexpr int PART_OFF = LSE_OFF + 8 * 2 * kRows * 4;  // [128] fp32
+  static constexpr int REC_OFF = PART_OFF + kKeys * 4;
   static constexpr int BAR_OFF = REC_OFF + kRecs * 48;
   static constexpr int META_OFF = BAR_OFF + 64 * 8;
-  static constexpr int SMEM = META_OFF + (kScMaxBatch + 1) * 4 + 1024;
+  static constexpr int SMEM = META_OFF + 5 * (kScMaxBatch + 1) * 4 + 1024;
 };
 
 // True for one lane of the (converged) warp, the same one each time.
@@ -91,12 +92,16 @@ __global__ void __launch_bounds__(kScThreads, 1)
   uint64_t *k_full = bars + 8, *k_empty = bars + 10;
   uint64_t *q_full = bars + 12, *q_empty = bars + 15;
   uint64_t *s_full = bars + 18, *s_free = bars + 22;   // [accumulator]
-  uint64_t *pt_full = bars + 26, *pt_free = bars + 38; // [group - 1][lane quarter]
-  uint64_t *drain = bars + 50;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 52);
+  uint64_t *pt_full = bars + 26, *pt_free = bars + 30; // [lane quarter]
+  uint64_t *drain = bars + 34;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 36);
   ScItem *recs = reinterpret_cast<ScItem *>(smem + L::REC_OFF);
   float *part = reinterpret_cast<float *>(smem + L::PART_OFF);
-  int *s_tiles = reinterpret_cast<int *>(smem + L::META_OFF);  // key tiles of each request
+  int *tiles_pre = reinterpret_cast<int *>(smem + L::META_OFF);
+  int *s_qo = tiles_pre + (kScMaxBatch + 1);
+  int *s_ip = s_qo + (kScMaxBatch + 1);
+  int *s_lk = s_ip + (kScMaxBatch + 1);
+  int *s_order = s_lk + (kScMaxBatch + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = p.group, tq = kRows / g, m_used = tq * g;
@@ -104,20 +109,47 @@ __global__ void __launch_bounds__(kScThreads, 1)
   // ---- once per CTA: key tiles per request, barriers, TMEM --------------------
   auto qo_at = [&](int i) { return min(max(p.qo_indptr[i], 0), p.total_q); };
   for (int i = threadIdx.x; i <= p.batch; i += blockDim.x) {
-    const int v = qo_at(i), next = i < p.batch ? qo_at(i + 1) : v;
-    if (blockIdx.x == 0 && (v != p.qo_indptr[i] || next < v)) flag(p.status, MI_STATUS_BAD_POSITION);
-    if (i < p.batch)
-      s_tiles[i] = next > v ? cdiv(kv_len_of(p.indptr, p.last, i, p.ps), kKeys) : 0;
+    const int v = qo_at(i);
+    if (blockIdx.x == 0 && (v != p.qo_indptr[i] || (i < p.batch && qo_at(i + 1) < v)))
+      flag(p.status, MI_STATUS_BAD_POSITION);
+    s_qo[i] = v;
+    s_ip[i] = p.indptr[i];
+    if (i < p.batch) s_lk[i] = kv_len_of(p.indptr, p.last, i, p.ps);
   }
-  if (warp == 1) {
+  __syncthreads();
+  // requests with the most keys first (ties by index), by counting
+  for (int i = threadIdx.x; i < p.batch; i += blockDim.x) {
+    int rank = i;
+    if (p.batch <= kScSortBatch) {
+      rank = 0;
+      for (int j = 0; j < p.batch; ++j)
+        rank += (s_lk[j] > s_lk[i] || (s_lk[j] == s_lk[i] && j < i)) ? 1 : 0;
+    }
+    s_order[rank] = i;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int carry = 0;
+    if (lane == 0) tiles_pre[0] = 0;
+    for (int base = 0; base < p.batch; base += 32) {
+      const int bb = base + lane;
+      const int rb = bb < p.batch ? s_order[bb] : 0;
+      int x = bb < p.batch && s_qo[rb + 1] > s_qo[rb] ? cdiv(s_lk[rb], kKeys) : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (bb < p.batch) tiles_pre[bb + 1] = carry + x;
+      carry += __shfl_sync(0xffffffffu, x, 31);
+    }
+  } else if (warp == 1) {
     if (lane == 0) {
       for (int i = 0; i < kRecs; ++i) {
         mbar_init(&it_full[i], 1);
-        mbar_init(&it_empty[i], 1 + 4 * kGroups);  // the MMA thread and the summing warps
+        mbar_init(&it_empty[i], 9);  // the MMA thread and the 8 summing warps
         mbar_init(&s_full[i], 1);
-        mbar_init(&s_free[i], 4 * kGroups);
-      }
-      for (int i = 0; i < 4 * (kGroups - 1); ++i) {
+        mbar_init(&s_free[i], 4);
         mbar_init(&pt_full[i], 1);
         mbar_init(&pt_free[i], 1);
       }
@@ -150,59 +182,33 @@ __global__ void __launch_bounds__(kScThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const int64_t n_items = static_cast<int64_t>(tiles_pre[p.batch]) * p.hkv;
   bool ok = true;
 
   if (warp == 0) {
     // ============================ producer ======================================
     const uint64_t pol_q = evict_last_policy(), pol_k = evict_first_policy();
     int kc = 0, qc = 0;  // K and Q tiles issued
-    // Items in falling order of the key tiles from theirs to the request's end
-    // (what a causal item's queries are as many as), then by request, then by
-    // head. Tiles with more than `e` after them: sum of max(0, tiles - e).
-    auto tiles_past = [&](int e) {
-      int x = 0;
-      for (int i = lane; i < p.batch; i += 32) x += max(0, s_tiles[i] - e);
-      return __reduce_add_sync(0xffffffffu, x);
-    };
-    int most = 0;  // the longest request's tiles
-    for (int i = lane; i < p.batch; i += 32) most = max(most, s_tiles[i]);
-    most = __reduce_max_sync(0xffffffffu, most);
-    const int64_t n_items = static_cast<int64_t>(tiles_past(0)) * p.hkv;
     for (int it = 0; ok; ++it) {
       int64_t k = 0;
       if (lane == 0) k = a.ctr ? atomicAdd(a.ctr, 1u) : blockIdx.x + int64_t(it) * gridDim.x;
       k = __shfl_sync(0xffffffffu, k, 0);
       ScItem rec{-1, 0, 0, 0, 0, 0, 0, 0, 0, 0, {0, 0}};
       if (k < n_items) {
-        const int tile = static_cast<int>(k / p.hkv);
-        // level e: the item's tile has e tiles after it; the least e with no
-        // more than `tile` tiles past it
-        int lo = 0, hi = most - 1;
+        int lo = 0, hi = p.batch - 1;  // last position with tiles_pre[pos] * hkv <= k
         while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (tiles_past(mid + 1) <= tile) hi = mid; else lo = mid + 1;
+          const int mid = (lo + hi + 1) >> 1;
+          if (static_cast<int64_t>(tiles_pre[mid]) * p.hkv <= k) lo = mid; else hi = mid - 1;
         }
-        const int e = lo;
-        int nth = tile - tiles_past(e + 1);  // of the requests with more than e tiles
-        int b = -1;
-        for (int base = 0; base < p.batch && b < 0; base += 32) {
-          const bool in = base + lane < p.batch && s_tiles[base + lane] > e;
-          const uint32_t m = __ballot_sync(0xffffffffu, in);
-          const int c = __popc(m);
-          if (nth < c) {
-            const uint32_t hit =
-                __ballot_sync(0xffffffffu, in && __popc(m & ((1u << lane) - 1u)) == nth);
-            b = base + __ffs(hit) - 1;
-          }
-          nth -= c;
-        }
+        const int b = s_order[lo];
+        const int rem = static_cast<int>(k - static_cast<int64_t>(tiles_pre[lo]) * p.hkv);
         rec.b = b;
-        rec.h = static_cast<int>(k % p.hkv);
-        rec.j0 = (s_tiles[b] - 1 - e) * kKeys;
-        rec.q_start = qo_at(b);
-        rec.nq = qo_at(b + 1) - rec.q_start;
-        rec.kvlen = kv_len_of(p.indptr, p.last, b, p.ps);
-        rec.page_base = p.indptr[b];
+        rec.h = rem % p.hkv;
+        rec.j0 = rem / p.hkv * kKeys;
+        rec.q_start = s_qo[b];
+        rec.nq = s_qo[b + 1] - rec.q_start;
+        rec.kvlen = s_lk[b];
+        rec.page_base = s_ip[b];
         rec.off = p.causal ? rec.kvlen - rec.nq : INT32_MAX / 2;
         rec.i0 = p.window > 0 ? max(0, rec.nq - p.window) : 0;
         if (p.causal) rec.i0 = max(rec.i0, rec.j0 - rec.off);
@@ -327,16 +333,20 @@ __global__ void __launch_bounds__(kScThreads, 1)
       if (!__all_sync(0xffffffffu, mbar_wait_bounded(drain, 0))) ok = false;
     }
   } else {
-    // ============================ sums (warps 2..17) =============================
-    const int wg = (warp - 2) >> 2;  // group
-    const int col0 = wg * kCols;     // its columns of a tile
+    // ============================ sums (warps 2..9) ==============================
+    const int wg = (warp - 2) >> 2;  // group: every other tile
     const int qd = warp & 3;         // the TMEM lane quarter this warp may access
     const int key = qd * 32 + lane;
-    float *lse_s = reinterpret_cast<float *>(smem + L::LSE_OFF) + (warp - 2) * 2 * kCols;
-    // row col0 + lane of a tile: query token and head offset
-    const int row = col0 + lane;
-    const int rt = row < m_used ? row / g : INT32_MAX / 2;
-    const int64_t ro = row < m_used ? static_cast<int64_t>(row / g) * p.hq + row % g : 0;
+    float *lse_s = reinterpret_cast<float *>(smem + L::LSE_OFF) + (warp - 2) * 2 * kRows;
+    // rows lane, lane + 32, ... of a tile: query token and head offset
+    int rt[4];
+    int64_t ro[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = lane + 32 * i;
+      rt[i] = r < m_used ? r / g : INT32_MAX / 2;
+      ro[i] = r < m_used ? static_cast<int64_t>(r / g) * p.hq + r % g : 0;
+    }
     int gt = 0, buf = 0, done = 0;
     for (int it = 0; ok; ++it) {
       const int slot = it % kRecs;
@@ -352,45 +362,51 @@ __global__ void __launch_bounds__(kScThreads, 1)
       const int j = rec.j0 + key;
       // row terms of tile t: log-sum-exp in log2 units; +inf for rows that are
       // not there or saw nothing, which makes their exp2 zero
-      float lv = 0.f;
+      float lv[4];
       auto load_lse = [&](int t) {
         const int tok = rec.i0 + t * tq;
-        lv = INFINITY;
-        if (rt < rec.nq - tok)
-          lv = p.lse[static_cast<int64_t>(rec.q_start + tok) * p.hq + rec.h * g + ro];
+        const float *l = p.lse + static_cast<int64_t>(rec.q_start + tok) * p.hq + rec.h * g;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          lv[i] = INFINITY;
+          if (rt[i] < rec.nq - tok) lv[i] = l[ro[i]];
+        }
       };
       float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-      load_lse(0);
-      for (int t = 0; t < rec.n_tiles; ++t) {
+      const int first = (gt & 1) == wg ? 0 : 1;  // tiles of this item that are this group's
+      if (first < rec.n_tiles) load_lse(first);
+      for (int t = first; t < rec.n_tiles; t += 2) {
         const int u = gt + t, acc = u % kAcc;
-        float *ls = lse_s + buf * kCols;
+        float *ls = lse_s + buf * kRows;
         buf ^= 1;
-        // (used here, a tile after its load: a use next to it would wait for it)
-        ls[lane] = lv == -INFINITY ? INFINITY : lv * kLog2e;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)  // (used here, a turn after its load, which no use waits for)
+          ls[lane + 32 * i] = lv[i] == -INFINITY ? INFINITY : lv[i] * kLog2e;
         __syncwarp();
-        if (t + 1 < rec.n_tiles) load_lse(t + 1);
+        if (t + 2 < rec.n_tiles) load_lse(t + 2);
         if (!__all_sync(0xffffffffu, mbar_wait_bounded(&s_full[acc], (u / kAcc) & 1))) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t ta = tmem + (static_cast<uint32_t>(qd * 32) << 16) + acc * kRows + col0;
+        const uint32_t ta = tmem + (static_cast<uint32_t>(qd * 32) << 16) + acc * kRows;
         const int tok = rec.i0 + t * tq;
-        // of this warp's columns, those of rows that are there and see this key:
-        // [cmin, cmax); past the last row that a full tile holds the terms are +inf
-        const int rows = min(tq, rec.nq - tok) * g;
-        const int cmax = rows - col0;
-        const int cmin = max(0, min(j - rec.off - tok, kRows)) * g - col0;
-        const bool full = __all_sync(0xffffffffu, cmin <= 0 && (rows == m_used || cmax >= kCols));
+        // columns of rows that are there and see this key: [cmin, cmax)
+        const int cmax = min(tq, rec.nq - tok) * g;
+        const int cmin = max(0, min(j - rec.off - tok, kRows)) * g;
+        const bool full = __all_sync(0xffffffffu, cmin == 0 && cmax == m_used);
         const float4 *l4 = reinterpret_cast<const float4 *>(ls);
-        if (!__all_sync(0xffffffffu, max(cmin, 0) >= min(cmax, kCols))) {
-          float x[kCols];
-          tmem_ld32(ta, x);
+        float v[2][32];
+        tmem_ld32(ta, v[0]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
           tmem_wait_ld();
+          if (c < 3) tmem_ld32(ta + (c + 1) * 32, v[(c + 1) & 1]);
+          const float *x = v[c & 1];
           if (full) {
 #pragma unroll
-            for (int i = 0; i < kCols; i += 4) {
-              const float4 l = l4[i / 4];
+            for (int i = 0; i < 32; i += 4) {
+              const float4 l = l4[c * 8 + i / 4];
               s0 += fast_exp2(fmaf(x[i], a.scale_log2, -l.x));
               s1 += fast_exp2(fmaf(x[i + 1], a.scale_log2, -l.y));
               s2 += fast_exp2(fmaf(x[i + 2], a.scale_log2, -l.z));
@@ -398,16 +414,17 @@ __global__ void __launch_bounds__(kScThreads, 1)
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < kCols; i += 4) {
-              const float4 l = l4[i / 4];
+            for (int i = 0; i < 32; i += 4) {
+              const float4 l = l4[c * 8 + i / 4];
+              const int col = c * 32 + i;
               const float e0 = fast_exp2(fmaf(x[i], a.scale_log2, -l.x));
               const float e1 = fast_exp2(fmaf(x[i + 1], a.scale_log2, -l.y));
               const float e2 = fast_exp2(fmaf(x[i + 2], a.scale_log2, -l.z));
               const float e3 = fast_exp2(fmaf(x[i + 3], a.scale_log2, -l.w));
-              s0 += i >= cmin && i < cmax ? e0 : 0.f;
-              s1 += i + 1 >= cmin && i + 1 < cmax ? e1 : 0.f;
-              s2 += i + 2 >= cmin && i + 2 < cmax ? e2 : 0.f;
-              s3 += i + 3 >= cmin && i + 3 < cmax ? e3 : 0.f;
+              s0 += col >= cmin && col < cmax ? e0 : 0.f;
+              s1 += col + 1 >= cmin && col + 1 < cmax ? e1 : 0.f;
+              s2 += col + 2 >= cmin && col + 2 < cmax ? e2 : 0.f;
+              s3 += col + 3 >= cmin && col + 3 < cmax ? e3 : 0.f;
             }
           }
         }
@@ -418,28 +435,22 @@ __global__ void __launch_bounds__(kScThreads, 1)
       if (!ok) break;
       gt += rec.n_tiles;
       const float s = (s0 + s1) + (s2 + s3);
-      if (wg > 0) {  // hand this group's sums to the first
-        const int pt = (wg - 1) * 4 + qd;
-        if (done > 0 && !__all_sync(0xffffffffu, mbar_wait_bounded(&pt_free[pt], (done - 1) & 1))) {
+      if (wg == 1) {  // hand this group's sums to the first
+        if (done > 0 && !__all_sync(0xffffffffu, mbar_wait_bounded(&pt_free[qd], (done - 1) & 1))) {
           ok = false;
           break;
         }
-        part[(wg - 1) * kKeys + key] = s;
+        part[key] = s;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&pt_full[pt]);
+        if (lane == 0) mbar_arrive(&pt_full[qd]);
       } else {
-        float sum = s;
-        for (int w = 1; w < kGroups; ++w) {
-          const int pt = (w - 1) * 4 + qd;
-          if (!__all_sync(0xffffffffu, mbar_wait_bounded(&pt_full[pt], done & 1))) {
-            ok = false;
-            break;
-          }
-          sum += part[(w - 1) * kKeys + key];
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&pt_free[pt]);
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&pt_full[qd], done & 1))) {
+          ok = false;
+          break;
         }
-        if (!ok) break;
+        const float sum = s + part[key];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pt_free[qd]);
         if (j < rec.kvlen) {
           const int64_t page = p.indices[rec.page_base + j / p.ps];
           if (page >= 0 && page < p.num_pages)
