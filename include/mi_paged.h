@@ -244,7 +244,9 @@ int mi_paged_prefill(
  *
  * mi_paged_decode_scores: mi_paged_decode (k_new NULL) or
  * mi_paged_decode_append (k_new given; same coverage, MI_ERR_UNSUPPORTED
- * otherwise) with the scores accumulated on the way: same out and lse.
+ * otherwise) with the scores accumulated on the way. Same out and lse, bit for
+ * bit where the workspace kernels serve the shape (16-bit types, head_dim 64 /
+ * 128, group <= 16), within fp32 rounding elsewhere.
  * rope_positions (optional, with k_new): the RoPE position of each request's
  * new token, which after an eviction is no longer its slot kv_len - 1.
  * max_pages: entries of kv_indices. scratch (256-byte aligned,

@@ -847,7 +847,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // others, combine the normalised partials of the runs that cover them
 // (slots first_run + b .. last_run + b), lanes over head_dim. The run range
 // comes from kv_indptr before the wait (metadata only); after it, the lse
-// and the partial rows of up to kBatch runs are loaded in one round.
+// and the partial rows of kBatch runs are loaded in one round, the next
+// round's under the arithmetic of this one.
 template <typename T, int D>
 __global__ void __launch_bounds__(64) decode_sk_merge_kernel(const SkParams p, int grid_runs) {
   constexpr int DPL = D / 32;
@@ -892,21 +893,22 @@ __global__ void __launch_bounds__(64) decode_sk_merge_kernel(const SkParams p, i
   float M = -INFINITY, wsum = 0.f, acc[DPL];
 #pragma unroll
   for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
-  for (int c0 = 0; c0 < nch; c0 += kBatch) {
-    // lse of runs c0 .. c0+kBatch-1 (one lane each) and their rows, all in flight
+  // lse of runs c0 .. c0+kBatch-1 (one lane each) and their rows, all in flight
+  auto load = [&](int c0, float &lc, float (&v)[kBatch][DPL]) {
     const int cl = c0 + lane;
-    const float lc = (lane < kBatch && cl < nch) ? __ldcg(lse_col + static_cast<int64_t>(cl) * p.hq)
-                                                 : -INFINITY;
-    float v[kBatch][DPL];
+    lc = (lane < kBatch && cl < nch) ? __ldcg(lse_col + static_cast<int64_t>(cl) * p.hq)
+                                     : -INFINITY;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
 #pragma unroll
       for (int i = 0; i < DPL; ++i)
         v[j][i] = (c0 + j < nch) ? __ldcg(o_col + (c0 + j) * o_step + i * 32) : 0.f;
-    // running rescale to the batch's max (online softmax over batches)
+  };
+  // running rescale to the batch's max (online softmax over batches)
+  auto add = [&](float lc, const float (&v)[kBatch][DPL]) {
     const float mb = warp_max(lc);
     const float mn = fmaxf(M, mb);
-    if (mn == -INFINITY) continue;
+    if (mn == -INFINITY) return;
     const float corr = exp2f(M - mn);  // 0 when M = -inf
     wsum *= corr;
 #pragma unroll
@@ -920,6 +922,17 @@ __global__ void __launch_bounds__(64) decode_sk_merge_kernel(const SkParams p, i
 #pragma unroll
       for (int i = 0; i < DPL; ++i) acc[i] += wj * v[j][i];
     }
+  };
+  // one batch ahead: a request cut into all 148 runs (one long context) is 19
+  // batches, whose round trips in turn took 20 us
+  float la, lb, va[kBatch][DPL], vb[kBatch][DPL];
+  load(0, la, va);
+  for (int c0 = 0; c0 < nch; c0 += 2 * kBatch) {
+    load(c0 + kBatch, lb, vb);  // (past the last run: zeros, no loads)
+    add(la, va);
+    if (c0 + kBatch >= nch) break;
+    load(c0 + 2 * kBatch, la, va);
+    add(lb, vb);
   }
   const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
   T *ob = static_cast<T *>(p.out) + (static_cast<int64_t>(b) * p.hq + qrow) * D;

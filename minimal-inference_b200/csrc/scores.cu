@@ -9,8 +9,9 @@
 //     every logit, so its score form stores them (fp32, log2 units; 1/16 of
 //     the bytes of K and V at 4 heads per KV head, and L2 resident) and
 //     weights_kernel turns them into weights once the row sums are known:
-//     no second pass over K. Shapes outside that kernel run the generic form
-//     after the decode.
+//     no second pass over K. fp32 and odd head sizes do the same in three
+//     plain kernels (logits by 16-token pieces, softmax and P V by row); other
+//     shapes run the generic prompt form after the decode.
 //   * A prompt's last `window` queries, whose log-sum-exp the prefill
 //     attention returned (scores_tc.cu for 16-bit types; the generic kernel
 //     here for any type and head_dim).
@@ -134,6 +135,150 @@ int launch_generic(const ScoreParams &p, int dtype, cudaStream_t s) {
   }
 }
 
+// ---- generic decode ---------------------------------------------------------
+// Logits of every token: the same work items and dot products as above, each
+// (token, query head) stored in log2 units at [hq][stride].
+template <typename T>
+__global__ void __launch_bounds__(kGTok *kGParts) logits_generic_kernel(
+    const ScoreParams p, float *logits, int64_t stride) {
+  extern __shared__ float s_k[];  // [16][d + 1]
+  const int total = p.indptr[p.batch] - p.indptr[0];
+  const int chunks = (p.ps + kGTok - 1) / kGTok;
+  const int64_t items = static_cast<int64_t>(total) * chunks * p.hkv;
+  const int tok = threadIdx.x % kGTok, part = threadIdx.x / kGTok;
+  for (int64_t it = blockIdx.x; it < items; it += gridDim.x) {
+    const int h = static_cast<int>(it % p.hkv);
+    const int chunk = static_cast<int>(it / p.hkv % chunks);
+    const int pos = static_cast<int>(it / p.hkv / chunks);
+    const int b = request_of(p.indptr, p.batch, pos);
+    const int slot0 = chunk * kGTok;
+    const int64_t at = static_cast<int64_t>(pos) * p.ps + slot0;  // in a row of logits
+    const int j0 = (pos - (p.indptr[b] - p.indptr[0])) * p.ps + slot0;
+    const int nt = min(min(kGTok, p.ps - slot0), kv_len_of(p.indptr, p.last, b, p.ps) - j0);
+    if (nt <= 0 || at + nt > stride) continue;
+    const int64_t page = p.indices[p.indptr[0] + pos];
+    const bool bad = page < 0 || page >= p.num_pages;
+    if (bad && threadIdx.x == 0) flag(p.status, MI_STATUS_BAD_PAGE);
+    __syncthreads();  // the previous item's readers are done
+    if (!bad) {
+      const T *kp = static_cast<const T *>(p.kv) +
+                    ((page * 2) * p.ps + slot0) * (static_cast<int64_t>(p.hkv) * p.d) +
+                    static_cast<int64_t>(h) * p.d;
+      for (int e = threadIdx.x; e < nt * p.d; e += blockDim.x) {
+        const int r = e / p.d, c = e % p.d;
+        s_k[r * (p.d + 1) + c] = Elt<T>::to(kp[static_cast<int64_t>(r) * p.hkv * p.d + c]);
+      }
+    }
+    __syncthreads();
+    if (tok < nt) {
+      const float *kr = s_k + tok * (p.d + 1);
+      for (int r = part; r < p.group; r += kGParts) {
+        const int hq = h * p.group + r;
+        float s = -INFINITY;  // a bad page's tokens are left out
+        if (!bad) {
+          const T *qr = static_cast<const T *>(p.q) + b * p.qsn + hq * p.qsh;
+          s = 0.f;
+          for (int c = 0; c < p.d; ++c) s = fmaf(Elt<T>::to(qr[c]), kr[c], s);
+          s *= p.scale * kLog2e;
+        }
+        logits[hq * stride + at + tok] = s;
+      }
+    }
+  }
+}
+
+// One CTA per (request, query head): maximum and sum of its logits, then P V
+// with a thread per element of head_dim and as many token streams as fit, 8
+// rows of V in flight each; the streams' sums are added in order.
+constexpr int kRowThreads = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads) row_generic_kernel(
+    const ScoreParams p, const float *logits, int64_t stride, T *out, float *lse, float *lse2) {
+  __shared__ float s_red[kRowThreads];
+  const int b = blockIdx.x, hq = blockIdx.y, h = hq / p.group;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int first = p.indptr[b] - p.indptr[0];
+  const int64_t base = static_cast<int64_t>(first) * p.ps;
+  const int n = static_cast<int>(
+      max(int64_t(0), min(int64_t(kv_len_of(p.indptr, p.last, b, p.ps)), stride - base)));
+  const float *x = logits + hq * stride + base;
+  float m = -INFINITY;
+  for (int t = tid; t < n; t += kRowThreads) m = fmaxf(m, x[t]);
+  m = warp_max(m);
+  if (lane == 0) s_red[warp] = m;
+  __syncthreads();
+  for (int i = 0; i < kRowThreads / 32; ++i) m = fmaxf(m, s_red[i]);
+  __syncthreads();
+  float l = 0.f;
+  if (m > -INFINITY)
+    for (int t = tid; t < n; t += kRowThreads) l += exp2f(x[t] - m);
+  l = warp_sum(l);
+  if (lane == 0) s_red[warp] = l;
+  __syncthreads();
+  l = 0.f;
+  for (int i = 0; i < kRowThreads / 32; ++i) l += s_red[i];
+  __syncthreads();
+  const float all = l > 0.f ? m + log2f(l) : -INFINITY;
+  if (tid == 0) {
+    lse2[b * p.hq + hq] = all;
+    if (lse) lse[b * p.hq + hq] = l > 0.f ? all * kLn2 : -INFINITY;
+  }
+  const int streams = max(1, kRowThreads / p.d);  // head_dim <= 256
+  const int c = tid % p.d, st = tid / p.d;
+  const int64_t row = static_cast<int64_t>(p.hkv) * p.d;
+  float acc = 0.f;
+  if (st < streams && l > 0.f) {
+    const T *v = static_cast<const T *>(p.kv) + p.ps * row + static_cast<int64_t>(h) * p.d + c;
+    const int32_t *table = p.indices + p.indptr[b];
+    constexpr int kAhead = 8;
+    for (int t0 = st; t0 < n; t0 += streams * kAhead) {
+      float w[kAhead], vv[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int t = t0 + i * streams;
+        w[i] = t < n ? x[t] : -INFINITY;
+        const int64_t page = t < n ? table[t / p.ps] : -1;
+        vv[i] = page >= 0 && page < p.num_pages
+                    ? Elt<T>::to(v[(page * 2 * p.ps + t % p.ps) * row]) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) acc = fmaf(exp2f(w[i] - m), vv[i], acc);
+    }
+  }
+  s_red[tid] = acc;
+  __syncthreads();
+  if (st == 0) {
+    for (int i = 1; i < streams; ++i) acc += s_red[i * p.d + c];
+    out[(static_cast<int64_t>(b) * p.hq + hq) * p.d + c] =
+        Elt<T>::from(l > 0.f ? acc / l : 0.f);
+  }
+}
+
+template <typename T>
+int launch_generic_decode_t(const ScoreParams &p, float *logits, int64_t stride, void *out,
+                            float *lse, float *lse2, cudaStream_t s) {
+  const int64_t items = stride / p.ps * ((p.ps + kGTok - 1) / kGTok) * p.hkv;
+  const int blocks = static_cast<int>(std::min<int64_t>(items, num_sms() * 8));
+  logits_generic_kernel<T><<<blocks, kGTok * kGParts, kGTok * (p.d + 1) * 4, s>>>(p, logits,
+                                                                                  stride);
+  int rc = check_launch("logits_generic_kernel");
+  if (rc) return rc;
+  row_generic_kernel<T><<<dim3(p.batch, p.hq), kRowThreads, 0, s>>>(
+      p, logits, stride, static_cast<T *>(out), lse, lse2);
+  return check_launch("row_generic_kernel");
+}
+
+int launch_generic_decode(const ScoreParams &p, int dtype, float *logits, int64_t stride,
+                          void *out, float *lse, float *lse2, cudaStream_t s) {
+  switch (dtype) {
+    case MI_DTYPE_F32: return launch_generic_decode_t<float>(p, logits, stride, out, lse, lse2, s);
+    case MI_DTYPE_F16: return launch_generic_decode_t<__half>(p, logits, stride, out, lse, lse2, s);
+    default:
+      return launch_generic_decode_t<__nv_bfloat16>(p, logits, stride, out, lse, lse2, s);
+  }
+}
+
 // ---- decode: stored logits to weights ----------------------------------------
 // One thread per (token, KV head): grid y = KV head, x strides over the page
 // positions' slots. Reads of a head's logits and the score additions are both
@@ -195,6 +340,7 @@ extern "C" int mi_paged_decode_scores(
   MI_REQUIRE(page_size > 0 && num_kv_heads > 0 && head_dim > 0 && head_dim <= 256 &&
                  num_pages > 0 && max_pages > 0,
              "decode_scores: bad pool geometry");
+  MI_REQUIRE(num_qo_heads <= 65535, "decode_scores: too many heads");
   MI_REQUIRE(num_qo_heads >= num_kv_heads && num_qo_heads % num_kv_heads == 0,
              "decode_scores: num_qo_heads %d is not a multiple of num_kv_heads %d", num_qo_heads,
              num_kv_heads);
@@ -215,8 +361,24 @@ extern "C" int mi_paged_decode_scores(
   float *row_lse = static_cast<float *>(scratch);  // [batch][hq]
   float *logits = reinterpret_cast<float *>(static_cast<unsigned char *>(scratch) +
                                             up256(size_t(batch_size) * num_qo_heads * 4));
-  if (decode_fast_shape(q, q_stride_b, q_stride_h, kv_data, out, head_dim, dtype, group,
-                        batch_size)) {
+  const int64_t stride = max_pages * page_size;
+  auto launch_weights = [&]() -> int {
+    const int64_t blocks = (stride + 255) / 256;
+    const int x = static_cast<int>(std::min<int64_t>(blocks, 16 * num_sms() / num_kv_heads + 1));
+    const cudaError_t e = launch_pdl(weights_kernel, dim3(x, num_kv_heads), dim3(256), 0, s,
+                                     static_cast<const float *>(logits), stride,
+                                     static_cast<const float *>(row_lse), kv_indptr, kv_indices,
+                                     kv_last_page_len, batch_size, group, num_qo_heads, page_size,
+                                     num_kv_heads, num_pages, scores);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return fail(MI_ERR_CUDA, "weights_kernel launch: %s", cudaGetErrorString(e));
+    }
+    return check_launch("weights_kernel");
+  };
+  const bool fast = decode_fast_shape(q, q_stride_b, q_stride_h, kv_data, out, head_dim, dtype,
+                                      group, batch_size);
+  if (fast) {
     SkArgs sk{q, q_stride_b, q_stride_h, kv_data, num_pages, page_size, num_kv_heads,
               head_dim, dtype, kv_indptr, kv_indices, kv_last_page_len, batch_size,
               num_qo_heads, sm_scale, out, lse, workspace, workspace_bytes, status, s};
@@ -234,35 +396,26 @@ extern "C" int mi_paged_decode_scores(
     }
     sk.logits = logits;
     sk.lse2 = row_lse;
-    sk.logit_stride = max_pages * page_size;
+    sk.logit_stride = stride;
     const int rc = launch_decode_sk(sk);
     if (rc > 0) return rc;
-    if (rc == 0) {
-      const int64_t blocks = (max_pages * page_size + 255) / 256;
-      const int x = static_cast<int>(std::min<int64_t>(blocks, 16 * num_sms() / num_kv_heads + 1));
-      const cudaError_t e = launch_pdl(weights_kernel, dim3(x, num_kv_heads), dim3(256), 0, s,
-                                       static_cast<const float *>(logits), sk.logit_stride,
-                                       static_cast<const float *>(row_lse), kv_indptr, kv_indices,
-                                       kv_last_page_len, batch_size, group, num_qo_heads,
-                                       page_size, num_kv_heads, num_pages, scores);
-      if (e != cudaSuccess) {
-        cudaGetLastError();
-        return fail(MI_ERR_CUDA, "weights_kernel launch: %s", cudaGetErrorString(e));
-      }
-      return check_launch("weights_kernel");
-    }
+    if (rc == 0) return launch_weights();
   }
   if (k_new)
     return fail(MI_ERR_UNSUPPORTED, "decode_scores: shape outside the fused append's coverage");
-  float *l = lse ? lse : row_lse;
-  const int rc = mi_paged_decode(q, q_stride_b, q_stride_h, kv_data, num_pages, page_size,
-                                 num_kv_heads, head_dim, dtype, kv_indptr, kv_indices,
-                                 kv_last_page_len, batch_size, num_qo_heads, sm_scale, out, l,
-                                 workspace, workspace_bytes, status, stream);
-  if (rc != MI_OK) return rc;
   ScoreParams p{q, q_stride_b, q_stride_h, nullptr, batch_size, kv_data, num_pages, page_size,
                 num_kv_heads, head_dim, kv_indptr, kv_indices, kv_last_page_len, batch_size,
-                num_qo_heads, group, 0, 0, sm_scale, l, scores, status};
+                num_qo_heads, group, 0, 0, sm_scale, nullptr, scores, status};
+  if (!fast) {
+    const int rc = launch_generic_decode(p, dtype, logits, stride, out, lse, row_lse, s);
+    return rc ? rc : launch_weights();
+  }
+  p.lse = lse ? lse : row_lse;
+  const int rc = mi_paged_decode(q, q_stride_b, q_stride_h, kv_data, num_pages, page_size,
+                                 num_kv_heads, head_dim, dtype, kv_indptr, kv_indices,
+                                 kv_last_page_len, batch_size, num_qo_heads, sm_scale, out,
+                                 lse ? lse : row_lse, workspace, workspace_bytes, status, stream);
+  if (rc != MI_OK) return rc;
   return launch_generic(p, dtype, s);
 }
 

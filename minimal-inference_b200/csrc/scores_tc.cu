@@ -11,7 +11,7 @@
 // takes 1024 clocks a tile; shared memory, which bounds the kernel, takes 512
 // for the operands of the 128 x 128 x 128 product, 512 for the row terms (a
 // clock per 32 lanes and column) and 256 for the Q tile's arrival. Measured
-// (16 prompts of 100-1500 tokens, 32/8 heads of 128): 96 us, 1.7 times that
+// (16 prompts of 100-1500 tokens, 32/8 heads of 128): 96 us, 1.4 times that
 // bound of 1280 clocks a tile. Tried without gain: quarters or halves of a
 // tile to a group, four groups, 256 keys to an item, K tiles an item ahead.
 //

@@ -100,7 +100,15 @@ def test_decode_scores(hq, hkv, d, ps, dtype, lens):
     want, want_lse = w.run(q, c["t_pool"], return_lse=True)
     out, lse = w.run(q, c["t_pool"], return_lse=True, scores=c["t_scores"])
     w.check_status()
-    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    if dtype != "float32" and d in (64, 128) and hq // hkv <= 16:
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    else:  # other kernels than run()'s: both within a few fp32 roundings and the output's own
+        half = torch.finfo(out.dtype).eps / 2
+        gap = (out.double() - want.double()).abs()
+        assert (gap <= 2 * half * want.double().abs() + 1e-4).all(), gap.max()
+        fin = torch.isfinite(want_lse)
+        assert torch.equal(fin, torch.isfinite(lse))
+        assert (lse[fin] - want_lse[fin]).abs().max() <= 1e-4
     scale = 1 / math.sqrt(d)
     add = _expected(c, lambda b, k: so.decode_weights(c["q"][b], k, scale))
     _check_scores(c, add, c["t_scores"], hq // hkv + max(lens) / 16, _mag(c["q"], c))
@@ -192,7 +200,8 @@ def test_decode_scores_with_append_and_positions(hq, hkv, d, ps, dtype):
     pool_c, pool_d = c["t_pool"].clone(), c["t_pool"].clone()
     a = w.run_with_append(q, pool_c, k, v, cos, sin)
     b = w.run_with_append(q, pool_d, k, v, cos, sin, scores=c["t_scores"].clone())
-    assert torch.equal(a, b) and torch.equal(pool_c, pool_d)
+    assert torch.equal(pool_c, pool_d)
+    assert torch.equal(a, b) or (dtype == "float32" and (a - b).abs().max() <= 1e-4)
 
 
 @pytest.mark.parametrize("hq,hkv,d,ps,dtype", SHAPES)
