@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kGTok *kGParts) logits_generic_kernel(
 // One CTA per (request, query head): maximum and sum of its logits, then P V
 // with a thread per element of head_dim and as many token streams as fit, 8
 // rows of V in flight each; the streams' sums are added in order.
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 1024;  // (with 256 a row of 500 tokens takes 20 us longer)
 
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) row_generic_kernel(
@@ -291,20 +291,26 @@ __global__ void __launch_bounds__(256) weights_kernel(
   const int h = blockIdx.y;
   const int base = indptr[0];
   const int64_t n = min(static_cast<int64_t>(indptr[batch] - base) * ps, stride);
-  pdl_wait();
+  bool waited = false;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    // the token's request and page, under the decode's last kernel
     const int pos = static_cast<int>(i / ps), slot = static_cast<int>(i % ps);
     const int b = request_of(indptr, batch, pos);
     const int first = indptr[b] - base;
-    if (static_cast<int64_t>(pos - first) * ps + slot >= kv_len_of(indptr, last, b, ps)) continue;
+    const bool real =
+        static_cast<int64_t>(pos - first) * ps + slot < kv_len_of(indptr, last, b, ps);
     const int64_t page = indices[base + pos];
-    if (page < 0 || page >= num_pages) continue;  // (flagged by the decode)
+    if (!waited) pdl_wait();
+    waited = true;
+    if (!real || page < 0 || page >= num_pages) continue;  // (a bad page: flagged by the decode)
     const float *lg = logits + static_cast<int64_t>(h) * group * stride + i;
     const float *l2 = lse2 + b * hq + h * group;
     float w = 0.f;
+#pragma unroll 8
     for (int g = 0; g < group; ++g) w += exp2f(lg[g * stride] - l2[g]);
     red_add(scores + (page * hkv + h) * ps + slot, w);
   }
+  if (!waited) pdl_wait();  // this grid ends after the decode's, whoever waits for it
 }
 
 size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
