@@ -27,8 +27,11 @@
 //      token would be the kernel's largest cost); where that does not decide,
 //      a second pass counts down to 2^-64 (nothing below 2^-45 can be drawn).
 //      The mass is summed in the same pass, with the exact 64-bit exponential
-//      within 2^-8, and below it with the hardware's exp2, whose 2^-22 of so
-//      little is as good;
+//      within 2^-8, and below it with the hardware's exp2: good to kMassError,
+//      which finds the bin. Where a top-p edge lies closer to the target than
+//      that, and for wide sets, one more pass sums the row in 64 bits (9 us at
+//      152064 tokens; in the division's own pass 6, but 3 more at 200 rows,
+//      which do not take it);
 //   3. if no more than kCap tokens lie at or above that bin (the usual case),
 //      they are gathered, one per thread, and every filter and the draw happen
 //      on that list with exact weights, each as a search for the token at which
@@ -46,9 +49,9 @@
 //
 // Bound by latency, not by its one read of the row: a row is a chain of
 // cluster barriers of 1-2 us with a few passes over shared memory between
-// them. Measured (CUDA graph): 12.3 us for 1 x 32768 and for 9 x 50257; 67.6
+// them. Measured (CUDA graph): 12.3 us for 1 x 32768 and for 9 x 50257; 76
 // us for 64 x 152064 bf16 (nucleus of 0.9; the rows whose nucleus is wide take
-// 50 us of it), 118 us for 200 x 152064 fp32 with mixed settings (1.03 TB/s;
+// 60 us of it), 119 us for 200 x 152064 fp32 with mixed settings (1.02 TB/s;
 // clusters of 8 with two CTAs per SM pass in 5.4 waves).
 #include <cooperative_groups.h>
 
@@ -76,6 +79,11 @@ constexpr int kNear = 256;       // bins of the first pass by mass: down to 2^-1
 constexpr float kNearX = 12.f;   // logits below the largest that it counts for top-k, at least
 constexpr int kShort = 128;      // lists up to this are searched as one
 constexpr float kExact = 128.f;  // exact weights down to 2^-8
+// Relative error of the mass that is summed with the hardware's exp2 below
+// 2^-8. Of a weight of 2^-o: three roundings of o, ln 2 * 3 * 2^-24 o; one of o
+// - 44, 2^-19 ln 2; exp2's own 2^-22: 1.25e-7 o + 1.6e-6. Tokens past 2^-20 are
+// at most 2^18 2^-20 of the largest one's mass, with o <= 64: 4.1e-6 + 2e-6.
+constexpr double kMassError = 1e-5;
 constexpr float kRound = 8388608.f;  // adding it rounds to an integer, in the low bits
 constexpr int kLimb = 15;        // histogram masses: three 15-bit limbs in 32-bit counters
 constexpr int kMaxSlice = (1 << 17) - 1;  // limb sums: 2^17 tokens * 2^15 stay below 2^32
@@ -236,6 +244,7 @@ struct Shared {
   u64 share[128];                   // a long list's sums per 128th
   u64 acc[4];                       // integer sums over the list; [3]: entries in pairs
   u64 cross;
+  int close;
   u64 scan[kSWarps];
   uint32_t warp_n[kSWarps];
   float warp_hi[kSWarps];
@@ -245,6 +254,7 @@ struct Shared {
   float maxv;
   double lsum;       // sum of exp(x - max), temperature 1
   double2 total[2];  // mass, and what of it the first pass counts, per search
+  double exact[2];   // mass of 64-bit exponentials alone
   u64 mass, over;
   uint32_t first;    // lowest token with the largest logit
   uint32_t list_n[2];
@@ -524,13 +534,16 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
   // The listed token at which the running sum of w, from `above` on and in
   // falling `order`, reaches the target (always one: the first, if none is
   // needed): its order. part: the entry's 128th, rising as the order falls.
-  auto crossing = [&](bool has, u64 order, u64 w, uint32_t part, u64 above, double target) {
+  // With a slack: sh.close if the token's edges are not that far from the target.
+  auto crossing = [&](bool has, u64 order, u64 w, uint32_t part, u64 above, double target,
+                      double slack = -1.0) {
     const bool shorts = listed <= kShort;
     __syncthreads();  // (an earlier call's result has been read)
     if (tid < 128) sh.share[tid] = 0;
     if (tid == 0) {
       sh.acc[3] = 0;
       sh.cross = 0;
+      sh.close = 0;
       sh.r_u32[0] = 0;
       sh.r_u64[0] = above;
     }
@@ -575,8 +588,11 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
         if (o.x > order) before += o.y;
       }
       if (w && static_cast<double>(before + w) >= target &&
-          (before == 0 || static_cast<double>(before) < target))
+          (before == 0 || static_cast<double>(before) < target)) {
         sh.cross = order;
+        sh.close = target - static_cast<double>(before) <= slack ||
+                   static_cast<double>(before + w) - target <= slack;
+      }
     }
     __syncthreads();
     return sh.cross;
@@ -586,6 +602,26 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (lane == 0 && v) atomicAdd(&sh.acc[slot], v);
+  };
+  // the row's mass in 64-bit exponentials (of what a first search left)
+  auto exact_mass = [&]() {
+    double s = 0.0;
+    for (int v = v0 + lane; v < v1; v += 32) {
+      const uint4 raw = *reinterpret_cast<const uint4 *>(keys + v * VEC);
+      const K *e = reinterpret_cast<const K *>(&raw);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float x = KO::raw(e[j]);
+        const double w = rw.scaled(x);
+        s += !cut || thr.takes(x, base + v * VEC - pad + j) ? w : 0.0;
+      }
+    }
+    s = block_sum(s, sh.dsum);
+    if (tid == 0) sh.exact[sel] = s;
+    cluster.sync();
+    double all = 0.0;
+    ranks(&sh.exact[sel], [&](int, double v) { all += v; });
+    return all;
   };
   // ordered key of the largest logit (its float maps back to the type's bits)
   auto key_of_max = [&]() -> uint32_t { return KO::key(KO::bits(rw.fmax_)); };
@@ -793,7 +829,11 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
           __syncthreads();
           want = top_p * static_cast<double>(sh.acc[0]);
         }
-        const u64 last = crossing(keep, c, w, part, 0, want);
+        u64 last = crossing(keep, c, w, part, 0, want, by_mass ? kMassError * total : -1.0);
+        if (sh.close) {
+          want = exact_mass() * top_p;
+          last = crossing(keep, c, w, part, 0, want);
+        }
         keep = keep && c >= last;
       }
       if (minw > 0.0) keep = keep && rw.scaled(KO::value(comp_key(c))) >= minw;
@@ -840,6 +880,8 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
       if (cut) lo = max(lo, composite(KO::key(KO::bits(thr.x)), thr.i));
     }
     if (lo > hi) continue;  // no token past the bins: all are kept
+    // (the edges of so many tokens lie closer than the mass is known)
+    if (by_mass) target = exact_mass() * top_p;
     // divide the range until its tokens fit the list; the first time also the
     // mass above it (the count above is known)
     u64 above_m = 0;

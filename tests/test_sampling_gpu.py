@@ -188,3 +188,34 @@ def test_repeatable_and_captured():
 def test_no_rows():
     x = torch.empty(0, 100, device="cuda", dtype=torch.bfloat16)
     assert sample_tokens(x, torch.empty(0, device="cuda")).shape == (0,)
+
+
+@pytest.mark.parametrize("style,temperature", [("wide", 1.518), ("wide", 0.9), ("list", 1.0),
+                                               ("list", 0.77)])
+def test_top_p_next_to_a_tokens_edge(style, temperature):
+    """p is the fp32 number nearest to the share of a prefix, so p times the
+    mass lies within 2^-25 of a token's edge, and the token after the prefix is
+    the vocabulary's last: with u next to 1 it is drawn exactly when it is kept."""
+    rows, vocab = 48, 30011
+    rng = np.random.default_rng(int(temperature * 1000))
+    x = rng.normal(size=(rows, vocab)).astype(np.float32) * np.float32(1 if style == "list" else 2.5)
+    if style == "list":  # some hundred tokens above 2^-8, the others near 2^-13
+        x = (x * 0.1 - 9.0 * temperature).astype(np.float32)
+        x[:, :300] = -np.abs(rng.normal(size=(rows, 300))) * 2 * temperature
+    p = np.zeros(rows, np.float32)
+    want = []
+    for r in range(rows):
+        n = 40 + 4 * r if style == "list" else 2000 + 300 * r
+        order = np.argsort(-x[r], kind="stable")
+        at = order[n]  # the token after the prefix trades places with the last one
+        x[r, at], x[r, -1] = x[r, -1], x[r, at]
+        d = x[r].astype(np.float64)
+        w = np.exp((d - d.max()) / float(np.float32(temperature)))
+        mass = np.cumsum(np.sort(w)[::-1])
+        p[r] = mass[n - 1] / mass[-1]
+        want.append(sample_row(x[r], 1 - 2.0 ** -24, float(np.float32(temperature)), 0,
+                               float(p[r]), 0.0)[0])
+    u = torch.full((rows,), 1.0, device="cuda")
+    got = sample_tokens(torch.from_numpy(x).cuda(), u, temperature, 0, torch.from_numpy(p).cuda())
+    assert got.tolist() == want
+    assert 8 < sum(t == vocab - 1 for t in want) < rows - 8  # both sides of the edge occur
