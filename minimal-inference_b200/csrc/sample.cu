@@ -23,15 +23,14 @@
 //      or above which everything that may be kept lies: token counts for
 //      top-k; for top-p counts times each bin's least or most weight, against
 //      p times the row's mass. Only the tokens within 2^-16 of the largest
-//      weight (for top-k, within 12 of the largest logit) are counted at first (most of a row's are not, and an atomic a
-//      token would be the kernel's largest cost); where that does not decide,
+//      weight (for top-k, within 12 of the largest logit) are counted at first
+//      (most of a row's are not, and an atomic a token would be the kernel's
+//      largest cost); where that does not decide,
 //      a second pass counts down to 2^-64 (nothing below 2^-45 can be drawn).
 //      The mass is summed in the same pass, with the exact 64-bit exponential
-//      within 2^-8, and below it with the hardware's exp2: good to kMassError,
-//      which finds the bin. Where a top-p edge lies closer to the target than
-//      that, and for wide sets, one more pass sums the row in 64 bits (9 us at
-//      152064 tokens; in the division's own pass 6, but 3 more at 200 rows,
-//      which do not take it);
+//      within 2^-8, and below it with the hardware's exp2, good to mass_error.
+//      Where a top-p edge may lie closer to the target than that, one more
+//      pass sums the row in 64 bits (9 us at 152064 tokens);
 //   3. if no more than kCap tokens lie at or above that bin (the usual case),
 //      they are gathered, one per thread, and every filter and the draw happen
 //      on that list with exact weights, each as a search for the token at which
@@ -49,9 +48,9 @@
 //
 // Bound by latency, not by its one read of the row: a row is a chain of
 // cluster barriers of 1-2 us with a few passes over shared memory between
-// them. Measured (CUDA graph): 12.3 us for 1 x 32768 and for 9 x 50257; 76
+// them. Measured (CUDA graph): 12.5 us for 1 x 32768, 14 for 9 x 50257; 70
 // us for 64 x 152064 bf16 (nucleus of 0.9; the rows whose nucleus is wide take
-// 60 us of it), 119 us for 200 x 152064 fp32 with mixed settings (1.02 TB/s;
+// 50 us of it), 121 us for 200 x 152064 fp32 with mixed settings (1.01 TB/s;
 // clusters of 8 with two CTAs per SM pass in 5.4 waves).
 #include <cooperative_groups.h>
 
@@ -74,16 +73,19 @@ constexpr int kMaxCluster = 8;   // portable cluster size
 constexpr int kIdxBits = 18;     // vocabulary <= 2^18
 constexpr uint32_t kIdxMask = (1u << kIdxBits) - 1;
 constexpr int kWeightBits = 44;  // the largest weight is 2^44
+constexpr double kOne = 1ull << kWeightBits;
 constexpr int kFine = 1024;      // bins of 1/16 of -log2 w (two per thread)
 constexpr int kNear = 256;       // bins of the first pass by mass: down to 2^-16
 constexpr float kNearX = 12.f;   // logits below the largest that it counts for top-k, at least
 constexpr int kShort = 128;      // lists up to this are searched as one
 constexpr float kExact = 128.f;  // exact weights down to 2^-8
-// Relative error of the mass that is summed with the hardware's exp2 below
-// 2^-8. Of a weight of 2^-o: three roundings of o, ln 2 * 3 * 2^-24 o; one of o
-// - 44, 2^-19 ln 2; exp2's own 2^-22: 1.25e-7 o + 1.6e-6. Tokens past 2^-20 are
-// at most 2^18 2^-20 of the largest one's mass, with o <= 64: 4.1e-6 + 2e-6.
-constexpr double kMassError = 1e-5;
+// Error of the mass M that is summed with the hardware's exp2, all of it below
+// 2^-8 of the largest weight: of a weight of 2^-o three roundings of o, 3 ln 2
+// 2^-24 o, and exp2's own 2^-22. The sum of w o is at most M log2(N / M) over N
+// tokens (uniform weights have the largest), M in units of the largest weight.
+__device__ __forceinline__ double mass_error(double m, int tokens) {
+  return m * (1.3e-7 * log2f(static_cast<float>(tokens * kOne / fmax(m, kOne * 1e-6))) + 2.5e-7);
+}
 constexpr float kRound = 8388608.f;  // adding it rounds to an integer, in the low bits
 constexpr int kLimb = 15;        // histogram masses: three 15-bit limbs in 32-bit counters
 constexpr int kMaxSlice = (1 << 17) - 1;  // limb sums: 2^17 tokens * 2^15 stay below 2^32
@@ -249,12 +251,14 @@ struct Shared {
   uint32_t warp_n[kSWarps];
   float warp_hi[kSWarps];
   u64 wsum[kSWarps];
-  double dsum[kSWarps], dsum2[kSWarps];
+  double dsum[kSWarps], dsum2[kSWarps], msum[3][kSWarps];
   // read by the other CTAs of the cluster, each written once before a barrier
   float maxv;
   double lsum;       // sum of exp(x - max), temperature 1
-  double2 total[2];  // mass, and what of it the first pass counts, per search
-  double exact[2];   // mass of 64-bit exponentials alone
+  // per search: mass from 64-bit exponentials, from exp2, and what of both the
+  // first pass counts
+  double masses[2][3];
+  double exact[2];   // all the mass from 64-bit exponentials alone
   u64 mass, over;
   uint32_t first;    // lowest token with the largest logit
   uint32_t list_n[2];
@@ -536,7 +540,7 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
   // needed): its order. part: the entry's 128th, rising as the order falls.
   // With a slack: sh.close if the token's edges are not that far from the target.
   auto crossing = [&](bool has, u64 order, u64 w, uint32_t part, u64 above, double target,
-                      double slack = -1.0) {
+                      float slack = -1.f) {
     const bool shorts = listed <= kShort;
     __syncthreads();  // (an earlier call's result has been read)
     if (tid < 128) sh.share[tid] = 0;
@@ -631,12 +635,10 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
     const bool by_mass = !(use_k && sel == 0);
     // -- 2. counts per bin, and the mass
     uint32_t *fine = sh.fine[sel];
-    double sum = 0.0;
-    float inside = 0.f;  // of the sum: what is counted, to fp32
+    double sum = 0.0, fast = 0.0;  // mass; of exp2s (in units of the largest)
+    float inside = 0.f;  // of it: what is counted, to fp32
     // weight at t sixteenths, for what lies below 2^-8 (t = inf: 0)
-    auto far = [](float t) {
-      return fast_exp2(fmaf(t, -0.0625f, static_cast<float>(kWeightBits)));
-    };
+    auto far = [](float t) { return fast_exp2(t * -0.0625f); };
     auto count = [&](float z) { atomicAdd(&fine[__float_as_uint(z) & (kFine - 1)], 1u); };
     const int window =
         by_mass ? kNear
@@ -670,7 +672,7 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
 #pragma unroll
           for (int j = 0; j < VEC; ++j) part += w[j];
         }
-        sum += part;
+        fast += part;
       }
       if (near && by_mass) {
 #pragma unroll
@@ -694,10 +696,23 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
       }
     }
     if (by_mass) {
-      const double d = block_sum(sum, sh.dsum), in = block_sum(inside, sh.dsum2);
-      if (tid == 0) sh.total[sel] = make_double2(d, in);
+      // the three sums over the CTA, in a fixed order, a thread each
+      double v[3] = {sum, fast, inside};
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+        if (lane == 0) sh.msum[i][warp] = v[i];
+      }
+      __syncthreads();
+      if (tid < 3) {
+        double d = 0.0;
+        for (int i = 0; i < kSWarps; ++i) d += sh.msum[tid][i];
+        sh.masses[sel][tid] = tid == 0 ? d : d * kOne;
+      }
     }
     double target = top_k, total = 0.0;
+    float unsure = -1.f;  // error of the target
     float beyond = 0.f;  // mass not counted
     int fb = kFine, fa = kFine;
     uint32_t above_n = 0, upto_n = 0;
@@ -717,12 +732,16 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
       }
       cluster.sync();
       if (by_mass && pass == 0) {
-        double in = 0.0;
-        ranks(&sh.total[sel], [&](int, double2 v) {
-          total += v.x;
-          in += v.y;
+        struct Masses { double slow, fast, in; };
+        double m = 0.0, in = 0.0;
+        ranks(reinterpret_cast<Masses *>(sh.masses[sel]), [&](int, Masses v) {
+          total += v.slow;
+          m += v.fast;
+          in += v.in;
         });
+        total += m;
         target = total * top_p;
+        unsure = static_cast<float>(mass_error(m, p.vocab));
         beyond = static_cast<float>(total - in);
       }
       // The first bin by which the prefix has certainly reached the target (fb),
@@ -829,7 +848,7 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
           __syncthreads();
           want = top_p * static_cast<double>(sh.acc[0]);
         }
-        u64 last = crossing(keep, c, w, part, 0, want, by_mass ? kMassError * total : -1.0);
+        u64 last = crossing(keep, c, w, part, 0, want, unsure);
         if (sh.close) {
           want = exact_mass() * top_p;
           last = crossing(keep, c, w, part, 0, want);
@@ -880,76 +899,86 @@ __global__ void __launch_bounds__(kSThreads, 2) sample_kernel(const SampleParams
       if (cut) lo = max(lo, composite(KO::key(KO::bits(thr.x)), thr.i));
     }
     if (lo > hi) continue;  // no token past the bins: all are kept
-    // (the edges of so many tokens lie closer than the mass is known)
-    if (by_mass) target = exact_mass() * top_p;
-    // divide the range until its tokens fit the list; the first time also the
-    // mass above it (the count above is known)
-    u64 above_m = 0;
-    double above = above_n;
+    // With the mass in 64 bits: at once where an eighth of the edges or more lie
+    // closer to the target than it is known (bin fb has the smallest tokens that
+    // may be one), else only after a search that ended so close.
+    const u64 lo0 = lo, hi0 = hi;
     bool all = false;  // the target is not reached: everything in the range is kept
-    for (uint32_t inside = UINT32_MAX; inside > kCap;) {
-      const int shift = max(0, 64 - __clzll(static_cast<long long>(hi - lo)) - 8);
-      for (int i = tid; i < kBins; i += kSThreads) sh.hist[level & 1][i] = Bin{0, 0, 0, 0};
-      __syncthreads();
-      u64 over = 0;
-      const bool first = inside == UINT32_MAX;
-      const Place least = place_of(lo), most = place_of(hi + 1);  // range: takes least, not most
-      each(
-          least.x,
-          [&](float x, uint32_t i) {
-            return least.takes(x, i) && ((by_mass && first) || !most.takes(x, i));
-          },
-          [&](float x, uint32_t i) {
-            const u64 w = by_mass ? rw.weight(x) : 0;
-            if (most.takes(x, i))
-              over += w;
-            else
-              add(static_cast<int>((hi - comp_of(x, i)) >> shift), by_mass, w);
-          });
-      if (by_mass && first) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) over += __shfl_xor_sync(0xffffffffu, over, o);
-        if (lane == 0) sh.wsum[warp] = over;
+    for (bool settle = by_mass && fast_exp2(-0.0625f * fb) * kOne < 16 * unsure;; settle = true) {
+      if (settle) {  // (its cluster barrier: every CTA has read the lists)
+        target = exact_mass() * top_p;
+        unsure = -1.f;
+        lo = lo0, hi = hi0;
+        if (tid == 0) sh.list_n[sel & 1] = 0;
+      }
+      // divide the range until its tokens fit the list; the first time also the
+      // mass above it (the count above is known)
+      u64 above_m = 0;
+      double above = above_n;
+      all = false;
+      for (uint32_t inside = UINT32_MAX; inside > kCap;) {
+        const int shift = max(0, 64 - __clzll(static_cast<long long>(hi - lo)) - 8);
+        for (int i = tid; i < kBins; i += kSThreads) sh.hist[level & 1][i] = Bin{0, 0, 0, 0};
         __syncthreads();
-        if (tid == 0) {
-          for (int i = 1; i < kSWarps; ++i) over += sh.wsum[i];
-          sh.over = over;
+        u64 over = 0;
+        const bool first = inside == UINT32_MAX;
+        const Place least = place_of(lo), most = place_of(hi + 1);  // range: takes least, not most
+        each(
+            least.x,
+            [&](float x, uint32_t i) {
+              return least.takes(x, i) && ((by_mass && first) || !most.takes(x, i));
+            },
+            [&](float x, uint32_t i) {
+              const u64 w = by_mass ? rw.weight(x) : 0;
+              if (most.takes(x, i))
+                over += w;
+              else
+                add(static_cast<int>((hi - comp_of(x, i)) >> shift), by_mass, w);
+            });
+        if (by_mass && first) {
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) over += __shfl_xor_sync(0xffffffffu, over, o);
+          if (lane == 0) sh.wsum[warp] = over;
+          __syncthreads();
+          if (tid == 0) {
+            for (int i = 1; i < kSWarps; ++i) over += sh.wsum[i];
+            sh.over = over;
+          }
         }
+        cluster.sync();
+        if (by_mass && first) {
+          ranks(&sh.over, [&](int, u64 v) { above_m += v; });
+          above = static_cast<double>(above_m);
+        }
+        merge(by_mass, target, above, above_m);
+        const uint32_t q = sh.r_u32[0];
+        if (q == kBins) {
+          all = true;
+          break;
+        }
+        above += sh.r_u32[1];  // (counts; by mass it is above_m that counts)
+        inside = sh.r_u32[2];
+        above_m += sh.r_u64[0];
+        if (by_mass) above = static_cast<double>(above_m);
+        __syncthreads();
+        hi -= static_cast<u64>(q) << shift;
+        const u64 width = (1ull << shift) - 1;
+        if (hi - lo > width) lo = hi - width;
       }
-      cluster.sync();
-      if (by_mass && first) {
-        ranks(&sh.over, [&](int, u64 v) { above_m += v; });
-        above = static_cast<double>(above_m);
-      }
-      merge(by_mass, target, above, above_m);
-      const uint32_t q = sh.r_u32[0];
-      if (q == kBins) {
-        all = true;
-        break;
-      }
-      above += sh.r_u32[1];  // (counts; by mass it is above_m that counts)
-      inside = sh.r_u32[2];
-      above_m += sh.r_u64[0];
-      if (by_mass) above = static_cast<double>(above_m);
-      __syncthreads();
-      hi -= static_cast<u64>(q) << shift;
-      const u64 width = (1ull << shift) - 1;
-      if (hi - lo > width) lo = hi - width;
+      if (all && unsure < 0.f) break;
+      if (all) continue;
+      const Place least = place_of(lo), most = place_of(hi + 1);
+      const u64 gc = gather(
+          least.x, [&](float x, uint32_t i) { return least.takes(x, i) && !most.takes(x, i); });
+      const u64 w = by_mass ? weight_of(gc) : (gc ? 1 : 0);
+      const int shift = max(0, 64 - __clzll(static_cast<long long>(hi - lo)) - 7);
+      const u64 last = crossing(gc != 0, gc, w, gc ? static_cast<uint32_t>((hi - gc) >> shift) : 0,
+                                by_mass ? above_m : static_cast<u64>(above), target, unsure);
+      if (sh.close && unsure >= 0.f) continue;
+      if (last) thr = place_of(last);
+      break;
     }
-    if (all) {
-      thr = place_of(lo);
-      cut = true;
-      __syncthreads();
-      continue;
-    }
-    const Place least = place_of(lo), most = place_of(hi + 1);
-    const u64 gc = gather(
-        least.x, [&](float x, uint32_t i) { return least.takes(x, i) && !most.takes(x, i); });
-    const u64 w = by_mass ? weight_of(gc) : (gc ? 1 : 0);
-    const int shift = max(0, 64 - __clzll(static_cast<long long>(hi - lo)) - 7);
-    const u64 last = crossing(gc != 0, gc, w, gc ? static_cast<uint32_t>((hi - gc) >> shift) : 0,
-                              by_mass ? above_m : static_cast<u64>(above), target);
-    if (last) thr = place_of(last);
+    if (all) thr = place_of(lo);
     cut = true;
     __syncthreads();
   }
