@@ -110,7 +110,8 @@ class PagedKVCache:
         t = torch.tensor(pages, dtype=torch.int32, device=self.device)
         if self.score_data is not None:
             own = [p for p in pages if 0 <= p < self.max_num_pages]  # others are flagged below
-            self.score_data.index_fill_(1, torch.tensor(own, device=self.device), 0.0)
+            self.score_data.index_fill_(
+                1, torch.tensor(own, dtype=torch.int64, device=self.device), 0.0)
         capi.call("mi_page_release", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
                   self.max_num_pages, t.data_ptr(), len(pages), self.layer_ptrs.data_ptr(),
                   self.num_layers, self.page_bytes, self.status.data_ptr(), stream_of(t))
