@@ -34,7 +34,7 @@ import math
 import torch
 
 from . import capi
-from ._tensor import dtype_code, need_i32, ptr, stream_of
+from ._tensor import dtype_code, need_i32, on_device_of, ptr, stream_of
 
 
 class _FreeCount:
@@ -78,13 +78,18 @@ class PagedKVCache:
         self.page_table = torch.full((max_batch_size, self.max_pages_per_seq), -1, **i32)
         self.slot_num_pages = torch.zeros(max_batch_size, **i32)
         self.status = torch.zeros(1, **i32)
-        capi.call("mi_page_pool_init", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
-                  self.max_num_pages, stream_of(self.free_ring))
+        self._call("mi_page_pool_init", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
+                   self.max_num_pages, stream_of(self.free_ring))
         # accumulated attention weights [layers, P, Hkv, ps], or None
         self.score_data = (torch.zeros(self.num_layers, self.max_num_pages, self.num_kv_heads,
                                        page_size, device=device) if track_scores else None)
         self.num_free_pages = self.max_num_pages - 1
         self.free_pages = _FreeCount(self)
+
+    def _call(self, name: str, *args) -> None:
+        """An entry point, launched on the cache's device whichever is current."""
+        with on_device_of(self.page_table):
+            capi.call(name, *args)
 
     # ---- reference list API ---------------------------------------------
     def allocate_pages(self, num_pages: int) -> list[int]:
@@ -96,9 +101,9 @@ class PagedKVCache:
             return []
         counts = torch.tensor([num_pages], dtype=torch.int32, device=self.device)
         out = torch.empty(num_pages, dtype=torch.int32, device=self.device)
-        capi.call("mi_page_alloc", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
-                  self.max_num_pages, counts.data_ptr(), 1, out.data_ptr(),
-                  self.status.data_ptr(), stream_of(out))
+        self._call("mi_page_alloc", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
+                   self.max_num_pages, counts.data_ptr(), 1, out.data_ptr(),
+                   self.status.data_ptr(), stream_of(out))
         self.num_free_pages -= num_pages
         return out.tolist()
 
@@ -112,9 +117,9 @@ class PagedKVCache:
             own = [p for p in pages if 0 <= p < self.max_num_pages]  # others are flagged below
             self.score_data.index_fill_(
                 1, torch.tensor(own, dtype=torch.int64, device=self.device), 0.0)
-        capi.call("mi_page_release", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
-                  self.max_num_pages, t.data_ptr(), len(pages), self.layer_ptrs.data_ptr(),
-                  self.num_layers, self.page_bytes, self.status.data_ptr(), stream_of(t))
+        self._call("mi_page_release", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
+                   self.max_num_pages, t.data_ptr(), len(pages), self.layer_ptrs.data_ptr(),
+                   self.num_layers, self.page_bytes, self.status.data_ptr(), stream_of(t))
         self.num_free_pages += len(pages)
 
     # ---- slot API (no host synchronisation) --------------------------------
@@ -123,10 +128,10 @@ class PagedKVCache:
         if self.num_free_pages < total:
             raise RuntimeError(
                 f"Cannot allocate {total} pages, only {self.num_free_pages} free")
-        capi.call("mi_slot_alloc", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
-                  self.max_num_pages, self.page_table.data_ptr(), self.slot_num_pages.data_ptr(),
-                  self.max_batch_size, self.max_pages_per_seq, slots.data_ptr(),
-                  counts.data_ptr(), slots.numel(), self.status.data_ptr(), stream_of(slots))
+        self._call("mi_slot_alloc", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
+                   self.max_num_pages, self.page_table.data_ptr(), self.slot_num_pages.data_ptr(),
+                   self.max_batch_size, self.max_pages_per_seq, slots.data_ptr(),
+                   counts.data_ptr(), slots.numel(), self.status.data_ptr(), stream_of(slots))
         self.num_free_pages -= total
 
     def slot_release(self, slots: torch.Tensor, total_pages: int) -> None:
@@ -134,22 +139,22 @@ class PagedKVCache:
         if self.score_data is not None:
             self._trim(slots, 0, total_pages)
             return
-        capi.call("mi_slot_release", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
-                  self.max_num_pages, self.page_table.data_ptr(), self.slot_num_pages.data_ptr(),
-                  self.max_batch_size, self.max_pages_per_seq, slots.data_ptr(), slots.numel(),
-                  self.layer_ptrs.data_ptr(), self.num_layers, self.page_bytes,
-                  self.status.data_ptr(), stream_of(slots))
+        self._call("mi_slot_release", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
+                   self.max_num_pages, self.page_table.data_ptr(), self.slot_num_pages.data_ptr(),
+                   self.max_batch_size, self.max_pages_per_seq, slots.data_ptr(), slots.numel(),
+                   self.layer_ptrs.data_ptr(), self.num_layers, self.page_bytes,
+                   self.status.data_ptr(), stream_of(slots))
         self.num_free_pages += total_pages
 
     def _trim(self, slots: torch.Tensor, keep_pages: int, freed_pages: int) -> None:
         """Free the pages of ``slots`` from the ``keep_pages``-th on, zeroed."""
         sc = self.score_data
-        capi.call("mi_slot_trim", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
-                  self.max_num_pages, self.page_table.data_ptr(), self.slot_num_pages.data_ptr(),
-                  self.max_batch_size, self.max_pages_per_seq, slots.data_ptr(), slots.numel(),
-                  keep_pages, self.layer_ptrs.data_ptr(), self.num_layers, self.page_bytes,
-                  ptr(sc), self.num_kv_heads * self.page_size, self.status.data_ptr(),
-                  stream_of(slots))
+        self._call("mi_slot_trim", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
+                   self.max_num_pages, self.page_table.data_ptr(), self.slot_num_pages.data_ptr(),
+                   self.max_batch_size, self.max_pages_per_seq, slots.data_ptr(), slots.numel(),
+                   keep_pages, self.layer_ptrs.data_ptr(), self.num_layers, self.page_bytes,
+                   ptr(sc), self.num_kv_heads * self.page_size, self.status.data_ptr(),
+                   stream_of(slots))
         self.num_free_pages += freed_pages
 
     def evict(self, slots: torch.Tensor, lengths: torch.Tensor, budget: int,
@@ -177,11 +182,11 @@ class PagedKVCache:
                                 torch.empty(n, **i32))
         indices = torch.empty(n * self.max_pages_per_seq, **i32)
         self.step_prepare(slots, lengths - 1, indptr, indices, last, unused, grow=False)
-        capi.call("mi_kv_evict", self.layer_ptrs.data_ptr(), None, 0, self.score_data.data_ptr(),
-                  self.num_layers, self.max_num_pages, self.page_size, self.num_kv_heads,
-                  self.head_dim, dtype_code(self.dtype), indptr.data_ptr(), indices.data_ptr(),
-                  last.data_ptr(), n, self.max_pages_per_seq * self.page_size, budget, recent,
-                  sinks, None, self.status.data_ptr(), stream_of(slots))
+        self._call("mi_kv_evict", self.layer_ptrs.data_ptr(), None, 0, self.score_data.data_ptr(),
+                   self.num_layers, self.max_num_pages, self.page_size, self.num_kv_heads,
+                   self.head_dim, dtype_code(self.dtype), indptr.data_ptr(), indices.data_ptr(),
+                   last.data_ptr(), n, self.max_pages_per_seq * self.page_size, budget, recent,
+                   sinks, None, self.status.data_ptr(), stream_of(slots))
         self._trim(slots, math.ceil(budget / self.page_size), freed_pages)
 
     def step_prepare(self, lane_slots: torch.Tensor, lane_positions: torch.Tensor,
@@ -193,13 +198,13 @@ class PagedKVCache:
         Graph-capturable. The caller accounts for grown pages in
         ``num_free_pages`` (it knows positions on the host).
         """
-        capi.call("mi_step_prepare", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
-                  self.max_num_pages, self.page_table.data_ptr(), self.slot_num_pages.data_ptr(),
-                  self.max_batch_size, self.max_pages_per_seq, lane_slots.data_ptr(),
-                  lane_positions.data_ptr(), lane_slots.numel(), self.page_size, int(grow),
-                  kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(),
-                  kv_last_page_len.data_ptr(), append_positions.data_ptr(),
-                  self.status.data_ptr(), stream_of(lane_slots))
+        self._call("mi_step_prepare", self.free_ring.data_ptr(), self.pool_ctrl.data_ptr(),
+                   self.max_num_pages, self.page_table.data_ptr(), self.slot_num_pages.data_ptr(),
+                   self.max_batch_size, self.max_pages_per_seq, lane_slots.data_ptr(),
+                   lane_positions.data_ptr(), lane_slots.numel(), self.page_size, int(grow),
+                   kv_indptr.data_ptr(), kv_indices.data_ptr(), kv_indices.numel(),
+                   kv_last_page_len.data_ptr(), append_positions.data_ptr(),
+                   self.status.data_ptr(), stream_of(lane_slots))
 
     def slot_pages(self, slot: int) -> list[int]:
         """Pages held by ``slot`` (reads the device table; synchronises)."""

@@ -38,3 +38,31 @@ def test_release_with_scores_reaches_the_pool(cache, pages, cleared):
     assert c.num_free_pages == 3 + len(pages)
     own = [p for p in range(8) if not c.score_data[:, p].any()]
     assert own == cleared
+
+
+def test_every_launch_is_made_on_the_caches_device(cache, monkeypatch):
+    """A stream handle does not name its device (every device's default stream is
+    handle 0), so the cache's device has to be the current one at each launch,
+    whichever is current at the call."""
+    c, _ = cache
+    current, calls = [], []
+
+    class On:
+        def __init__(self, t):
+            self.t = t
+
+        def __enter__(self):
+            current.append(self.t.device)
+
+        def __exit__(self, *a):
+            current.pop()
+
+    monkeypatch.setattr(kv_cache, "on_device_of", On)
+    monkeypatch.setattr(kv_cache.capi, "call",
+                        lambda name, *a: calls.append((name, bool(current))))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    c.evict(i32([0, 1]), i32([40, 20]), 16, 3, recent=4)
+    c.slot_release(i32([0]), 1)
+    c.release_pages([3])
+    assert calls == [(n, True) for n in ("mi_step_prepare", "mi_kv_evict", "mi_slot_trim",
+                                         "mi_slot_trim", "mi_page_release")]
