@@ -162,9 +162,10 @@ class PagedKVCache:
         """Cut each of ``slots`` (holding ``lengths`` tokens, both device int32)
         to at most ``budget`` tokens by accumulated score, in every layer and KV
         head (``page.evict_paged_kv_cache``), and free the pages past the
-        budget. ``slots`` must be distinct. ``freed_pages``: how many that is over all slots (the caller
-        knows the lengths). A slot's next token goes to position ``min(length,
-        budget)`` of its pages. Does not synchronise."""
+        budget. ``slots`` must be distinct. ``freed_pages``: how many that is
+        over all slots (the caller knows the lengths). A slot's next token goes
+        to position ``min(length, budget)`` of its pages. Does not
+        synchronise."""
         if self.score_data is None:
             raise RuntimeError("evict() needs PagedKVCache(track_scores=True)")
         if budget < 1 or recent < 0 or sinks < 0 or recent + sinks > budget:
@@ -181,7 +182,8 @@ class PagedKVCache:
         indptr, last, unused = (torch.empty(n + 1, **i32), torch.empty(n, **i32),
                                 torch.empty(n, **i32))
         indices = torch.empty(n * self.max_pages_per_seq, **i32)
-        self.step_prepare(slots, lengths - 1, indptr, indices, last, unused, grow=False)
+        lanes = torch.where(lengths > 0, slots, -1)  # an empty slot: a padding lane
+        self.step_prepare(lanes, lengths - 1, indptr, indices, last, unused, grow=False)
         self._call("mi_kv_evict", self.layer_ptrs.data_ptr(), None, 0, self.score_data.data_ptr(),
                    self.num_layers, self.max_num_pages, self.page_size, self.num_kv_heads,
                    self.head_dim, dtype_code(self.dtype), indptr.data_ptr(), indices.data_ptr(),

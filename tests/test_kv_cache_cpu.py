@@ -66,3 +66,16 @@ def test_every_launch_is_made_on_the_caches_device(cache, monkeypatch):
     c.release_pages([3])
     assert calls == [(n, True) for n in ("mi_step_prepare", "mi_kv_evict", "mi_slot_trim",
                                          "mi_slot_trim", "mi_page_release")]
+
+
+def test_evict_passes_an_empty_slot_over(cache, monkeypatch):
+    """A slot without tokens has no newest one: it goes in as a padding lane, not
+    as position -1, which the device would flag."""
+    c, _ = cache
+    seen = []
+    monkeypatch.setattr(c, "step_prepare", lambda slots, pos, *a, **k: seen.append(
+        (slots.tolist(), pos.tolist())))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    c.evict(i32([1, 0]), i32([0, 40]), 16, 2)
+    (slots, pos), = seen
+    assert slots[0] == -1 and slots[1] == 0 and pos[1] == 39
