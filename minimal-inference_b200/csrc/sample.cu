@@ -81,10 +81,12 @@ constexpr int kShort = 128;      // lists up to this are searched as one
 constexpr float kExact = 128.f;  // exact weights down to 2^-8
 // Error of the mass M that is summed with the hardware's exp2, all of it below
 // 2^-8 of the largest weight: of a weight of 2^-o three roundings of o, 3 ln 2
-// 2^-24 o, and exp2's own 2^-22. The sum of w o is at most M log2(N / M) over N
-// tokens (uniform weights have the largest), M in units of the largest weight.
+// 2^-24 o, exp2's own 2^-22, and the seven fp32 additions of a vector's eight
+// weights, 7 2^-24 (vectors are summed in 64 bits). The sum of w o is at most
+// M log2(N / M) over N tokens (uniform weights have the largest), M in units of
+// the largest weight.
 __device__ __forceinline__ double mass_error(double m, int tokens) {
-  return m * (1.3e-7 * log2f(static_cast<float>(tokens * kOne / fmax(m, kOne * 1e-6))) + 2.5e-7);
+  return m * (1.3e-7 * log2f(static_cast<float>(tokens * kOne / fmax(m, kOne * 1e-6))) + 6.6e-7);
 }
 constexpr float kRound = 8388608.f;  // adding it rounds to an integer, in the low bits
 constexpr int kLimb = 15;        // histogram masses: three 15-bit limbs in 32-bit counters
