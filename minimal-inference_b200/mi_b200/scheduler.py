@@ -467,16 +467,32 @@ class Scheduler:
                          and r.cached_len > self.kv_budget])
 
     def _sample(self, rows: torch.Tensor, reqs: list) -> list[int]:
-        """Next tokens of ``rows [B, V]``; temperature alone goes through
-        ``sample_rows`` as the reference's does, anything more through
-        ``sample_tokens``. -1: a row without a logit above -inf."""
-        if all(r.plain_sampling for r in reqs):
+        """Next tokens of ``rows [B, V]``: requests with temperature alone go
+        through ``sample_rows`` as the reference's do, those that ask for more
+        through ``sample_tokens``, whoever else is in the batch. -1: a row of
+        the latter without a logit above -inf."""
+        plain = [i for i, r in enumerate(reqs) if r.plain_sampling]
+        if len(plain) == len(reqs):
             return sample_rows(rows, [r.temperature for r in reqs]).tolist()
-        shared = torch.rand(len(reqs))  # torch's generator, as sample_rows uses
+        if not plain:
+            return self._sample_filtered(rows, reqs).tolist()
+        other = [i for i, r in enumerate(reqs) if not r.plain_sampling]
+        tokens = torch.empty(len(reqs), dtype=torch.long, device=rows.device)
+        tokens[plain] = sample_rows(rows[plain], [reqs[i].temperature for i in plain])
+        tokens[other] = self._sample_filtered(rows[other], [reqs[i] for i in other]).long()
+        return tokens.tolist()
+
+    def _sample_filtered(self, rows: torch.Tensor, reqs: list) -> torch.Tensor:
+        """``sample_tokens`` with the requests' settings; fills token_logprobs.
+        Requests without a seed draw from torch's generator on the device, the
+        one that ``sample_rows`` draws from."""
         floats = torch.tensor([
-            [float(u) if r.seed is None else r.next_uniform() for r, u in zip(reqs, shared)],
+            [0.0 if r.seed is None else r.next_uniform() for r in reqs],
             [r.temperature for r in reqs], [r.top_p for r in reqs], [r.min_p for r in reqs]],
             dtype=torch.float32).to(self.device)
+        unseeded = [i for i, r in enumerate(reqs) if r.seed is None]
+        if unseeded:
+            floats[0, unseeded] = torch.rand(len(unseeded), device=self.device)
         top_k = torch.tensor([min(max(r.top_k, 0), rows.shape[1]) for r in reqs],
                              dtype=torch.int32, device=self.device)
         tokens, logprobs = sample_tokens(rows, floats[0], floats[1], top_k, floats[2], floats[3],
@@ -485,7 +501,7 @@ class Scheduler:
             for r, lp in zip(reqs, logprobs.tolist()):
                 if r.logprobs:
                     r.token_logprobs.append(lp)
-        return tokens.tolist()
+        return tokens
 
     @staticmethod
     def _fail(req) -> None:
