@@ -498,8 +498,8 @@ class Scheduler:
         tokens, logprobs = sample_tokens(rows, floats[0], floats[1], top_k, floats[2], floats[3],
                                          return_logprobs=True)
         if any(r.logprobs for r in reqs):
-            for r, lp in zip(reqs, logprobs.tolist()):
-                if r.logprobs:
+            for r, tok, lp in zip(reqs, tokens.tolist(), logprobs.tolist()):
+                if r.logprobs and tok >= 0:
                     r.token_logprobs.append(lp)
         return tokens
 

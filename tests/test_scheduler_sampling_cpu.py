@@ -71,3 +71,11 @@ def test_unseeded_draws_repeat_with_torchs_generator(sched):
     b = draw()
     assert a[:2] == b[:2] and draw()[:2] != a[:2]
     assert a[2] == b[2]  # a seeded request's own numbers
+
+
+def test_a_request_that_ends_without_a_token_has_no_log_probability_of_it(sched):
+    rows = torch.full((2, 20), -math.inf)
+    rows[1, 3] = 0.0
+    reqs = [_req("nothing", 1.0, logprobs=True), _req("one", 1.0, logprobs=True)]
+    assert sched._sample(rows, reqs) == [-1, 3]
+    assert reqs[0].token_logprobs == [] and reqs[1].token_logprobs == [0.0]
