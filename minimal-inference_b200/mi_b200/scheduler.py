@@ -41,6 +41,7 @@ from collections import deque
 from dataclasses import dataclass, field
 
 import torch
+import torch.distributed as dist
 import torch.nn.functional as F
 
 from .decode import BatchDecodeWithPagedKVCacheWrapper
@@ -473,19 +474,26 @@ class Scheduler:
         the latter without a logit above -inf."""
         plain = [i for i, r in enumerate(reqs) if r.plain_sampling]
         if len(plain) == len(reqs):
-            return sample_rows(rows, [r.temperature for r in reqs]).tolist()
-        if not plain:
-            return self._sample_filtered(rows, reqs).tolist()
+            return self._agree(sample_rows(rows, [r.temperature for r in reqs]), reqs).tolist()
         other = [i for i, r in enumerate(reqs) if not r.plain_sampling]
-        tokens = torch.empty(len(reqs), dtype=torch.long, device=rows.device)
-        tokens[plain] = sample_rows(rows[plain], [reqs[i].temperature for i in plain])
-        tokens[other] = self._sample_filtered(rows[other], [reqs[i] for i in other]).long()
-        return tokens.tolist()
+        # tokens and log-probabilities (64 bits hold both exactly)
+        picked = torch.zeros(2, len(reqs), dtype=torch.float64, device=rows.device)
+        if plain:
+            picked[0, plain] = sample_rows(
+                rows[plain], [reqs[i].temperature for i in plain]).double()
+        picked[:, other] = self._sample_filtered(rows[other] if plain else rows,
+                                                 [reqs[i] for i in other])
+        tokens, logprobs = self._agree(picked, reqs).tolist()
+        tokens = [int(t) for t in tokens]
+        for req, tok, lp in zip(reqs, tokens, logprobs):
+            if req.logprobs and tok >= 0:
+                req.token_logprobs.append(lp)
+        return tokens
 
     def _sample_filtered(self, rows: torch.Tensor, reqs: list) -> torch.Tensor:
-        """``sample_tokens`` with the requests' settings; fills token_logprobs.
-        Requests without a seed draw from torch's generator on the device, the
-        one that ``sample_rows`` draws from."""
+        """``sample_tokens`` with the requests' settings -> ``[2, B]``: tokens,
+        log-probabilities. Requests without a seed draw from torch's generator
+        on the device, the one that ``sample_rows`` draws from."""
         floats = torch.tensor([
             [0.0 if r.seed is None else r.next_uniform() for r in reqs],
             [r.temperature for r in reqs], [r.top_p for r in reqs], [r.min_p for r in reqs]],
@@ -497,11 +505,19 @@ class Scheduler:
                              dtype=torch.int32, device=self.device)
         tokens, logprobs = sample_tokens(rows, floats[0], floats[1], top_k, floats[2], floats[3],
                                          return_logprobs=True)
-        if any(r.logprobs for r in reqs):
-            for r, tok, lp in zip(reqs, tokens.tolist(), logprobs.tolist()):
-                if r.logprobs and tok >= 0:
-                    r.token_logprobs.append(lp)
-        return tokens
+        return torch.stack([tokens.double(), logprobs.double()])
+
+    def _agree(self, picked: torch.Tensor, reqs: list) -> torch.Tensor:
+        """Under tensor parallelism the choice of the group's first rank, on every
+        rank: each rank draws from its own generator, and ranks that went on with
+        different tokens would mix different sequences in their all-reduces.
+        (Greedy choices are the same on all: the logits are.)"""
+        if getattr(self.model, "tp_size", 1) > 1 and any(r.temperature > 0 for r in reqs):
+            group = self.model.tp_group
+            src = dist.get_global_rank(group, 0) if group is not None else 0
+            picked = picked.contiguous()
+            dist.broadcast(picked, src=src, group=group)
+        return picked
 
     @staticmethod
     def _fail(req) -> None:
