@@ -14,7 +14,8 @@
 // head instead of the whole cache.
 //
 // One CTA per (layer, request, head). The scores are read once, as ordered bits
-// in shared memory (requests past kKeyCap tokens read them again each pass).
+// in shared memory (those of requests with no room for them there are read again
+// in each pass).
 // The threshold is found by radix select, 11 bits a pass: the first digit then
 // has two bits of mantissa, and a few hundred scores of like size do not all
 // meet in one counter. A bit per token in shared memory with running counts
@@ -38,8 +39,16 @@ constexpr int kEThreads = 256;
 constexpr int kEWarps = kEThreads / 32;
 constexpr int kRows = 8;       // row pairs a warp holds in registers while they move
 constexpr int kDigit = 11;     // radix select: 11, 11 and 10 bits
-constexpr int kKeyCap = 4096;  // tokens whose ordered scores are kept in shared memory
 constexpr int kESmemMax = 200 * 1024;
+// Room for the requests' ordered scores beside their bits, 4.25 bytes a token.
+// Where max_len says that all fit while four CTAs do on an SM (56 KB each, 12.1
+// KB of it static: 10360 tokens), that much: 64 requests of 8192 -> 8000 take 91
+// us, and 128 with the scores read again in each pass. Else (longer requests, or
+// a bound that says little, as a whole page table's) what leaves four CTAs' SM
+// 92 KB of L1, 6504 tokens: with 28 KB of L1 the rows' moves are slower (8 of up to
+// 4096 -> 1024 by their table's bound: 58 us for 48).
+constexpr int kESmemFour = 43 * 1024;
+constexpr int kESmemSome = 27 * 1024;
 
 struct EvictParams {
   void *const *layer_kv;  // pointer per layer, or null: kv + layer * kv_stride bytes
@@ -50,7 +59,7 @@ struct EvictParams {
   int64_t num_pages;
   int ps, hkv, row_bytes;  // row: one head of one token of K (or V)
   const int32_t *indptr, *indices, *last;
-  int batch, budget, recent, sinks, max_len, key_cap;
+  int batch, budget, recent, sinks, max_len, smem;
   int32_t *kept;
   int32_t *status;
 };
@@ -136,8 +145,8 @@ __global__ void __launch_bounds__(kEThreads, 4) evict_kernel(const EvictParams p
 
   const int words = (n + 31) / 32;
   uint32_t *bits = s_dyn, *before = s_dyn + words;  // kept tokens in earlier words
-  uint32_t *keys = s_dyn + (p.max_len + 31) / 32 * 2;
-  const bool held = n <= p.key_cap;
+  uint32_t *keys = before + words;
+  const bool held = (2 * words + n) * 4 <= p.smem;  // (else: read again in each pass)
   auto key_of = [&](int t) { return held ? keys[t] : score_key(*score_at(t)); };
   if (held && want > 0) {
     for (int t = sinks + tid; t < mid_end; t += kEThreads) keys[t] = score_key(*score_at(t));
@@ -343,11 +352,11 @@ __global__ void __launch_bounds__(kEThreads, 4) evict_kernel(const EvictParams p
 }
 
 template <typename V>
-int launch_evict(const EvictParams &p, int layers, int smem, cudaStream_t s) {
+int launch_evict(const EvictParams &p, int layers, cudaStream_t s) {
   static std::atomic<unsigned long long> attr_set{0};
   if (smem_limit_once(attr_set, evict_kernel<V>, kESmemMax) != cudaSuccess)
     return check_launch("evict_kernel smem attribute");
-  evict_kernel<V><<<dim3(p.batch * p.hkv, layers), kEThreads, smem, s>>>(p);
+  evict_kernel<V><<<dim3(p.batch * p.hkv, layers), kEThreads, p.smem, s>>>(p);
   return check_launch("evict_kernel");
 }
 
@@ -387,16 +396,16 @@ extern "C" int mi_kv_evict(void *const *layer_pools, void *kv_data, int64_t kv_l
                 num_pages * num_kv_heads * page_size, num_pages, page_size, num_kv_heads,
                 static_cast<int>(row), kv_indptr, kv_indices, kv_last_page_len, batch_size, budget,
                 recent, sinks, static_cast<int>(std::min<int64_t>(max_len, cap)), 0, kept, status};
-  const int map = (p.max_len + 31) / 32 * 8;
-  p.key_cap = std::min({p.max_len, kKeyCap, (kESmemMax - map) / 4});
-  const int smem = map + p.key_cap * 4;
+  const int map = (p.max_len + 31) / 32 * 8;  // the longest request's
+  const int64_t full = map + int64_t(p.max_len) * 4;
+  p.smem = full <= kESmemFour ? static_cast<int>(full) : std::max(map, kESmemSome);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   // torch's pools are 256-byte aligned; a caller's own need only be aligned to
   // the element, and then the copies are narrower. (With layer_pools the
   // pointers are on the device: mi_page_release already asks 16 bytes of them.)
   const bool wide = row % 16 == 0 && (layer_pools || (reinterpret_cast<uintptr_t>(kv_data) % 16 == 0 &&
                                                       p.kv_stride % 16 == 0));
-  if (wide) return launch_evict<uint4>(p, num_layers, smem, s);
-  if (es == 4) return launch_evict<uint32_t>(p, num_layers, smem, s);
-  return launch_evict<uint16_t>(p, num_layers, smem, s);
+  if (wide) return launch_evict<uint4>(p, num_layers, s);
+  if (es == 4) return launch_evict<uint32_t>(p, num_layers, s);
+  return launch_evict<uint16_t>(p, num_layers, s);
 }

@@ -109,7 +109,9 @@ def evict_paged_kv_cache(paged_kv_cache: torch.Tensor, scores: torch.Tensor,
     are 0 behind. The page table tensors are not changed.
 
     ``max_len``: an upper bound of the requests' lengths (default: all of
-    ``kv_indices``' slots; at most 819200). Returns, with ``return_kept``, int32
+    ``kv_indices``' slots; at most 819200). It sizes the shared memory: with a
+    large page table the longest request's length is the faster one to pass.
+    Returns, with ``return_kept``, int32
     ``[(L,) B, Hkv, budget]``: the slot each kept token came from (-1: none)."""
     stacked = paged_kv_cache.dim() == 6
     layers = paged_kv_cache.shape[0] if stacked else 1
