@@ -100,7 +100,8 @@ struct SkParams {
   // Score form (mi_paged_decode_scores): the scaled logits (log2 units) of
   // every token under every query head, [hq][logit_stride] with a request's
   // tokens at (its first page position) * ps onward, and the rows'
-  // log2-sum-exp; decode_scores.cu turns them into weights afterwards.
+  // log2-sum-exp (+inf for a row without a weight, so that exp2 of the
+  // difference is 0); scores.cu turns them into weights afterwards.
   float *logits, *lse2;
   int64_t logit_stride;
   const int32_t *rope_pos;  // optional RoPE position of each request's new token
@@ -824,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (p.lse && lane == 0)
           p.lse[b * p.hq + qrow] = L > 0.f ? (M + __log2f(L)) * kLn2 : -INFINITY;
         if constexpr (SCORES) {
-          if (lane == 0) p.lse2[b * p.hq + qrow] = L > 0.f ? M + log2f(L) : -INFINITY;
+          if (lane == 0) p.lse2[b * p.hq + qrow] = L > 0.f ? M + log2f(L) : INFINITY;
         }
       } else {
         float *po = p.part_o + (static_cast<int64_t>(slot) * p.hq + qrow) * D;
@@ -941,7 +942,7 @@ __global__ void __launch_bounds__(64) decode_sk_merge_kernel(const SkParams p, i
   if (p.lse && lane == 0)
     p.lse[b * p.hq + qrow] = wsum > 0.f ? (M + __log2f(wsum)) * kLn2 : -INFINITY;
   if (p.lse2 && lane == 0)
-    p.lse2[b * p.hq + qrow] = wsum > 0.f ? M + log2f(wsum) : -INFINITY;
+    p.lse2[b * p.hq + qrow] = wsum > 0.f ? M + log2f(wsum) : INFINITY;
 }
 
 // ---------------------------------------------------------------------------

@@ -221,9 +221,9 @@ __global__ void __launch_bounds__(kRowThreads) row_generic_kernel(
   l = 0.f;
   for (int i = 0; i < kRowThreads / 32; ++i) l += s_red[i];
   __syncthreads();
-  const float all = l > 0.f ? m + log2f(l) : -INFINITY;
+  const float all = m + log2f(l);
   if (tid == 0) {
-    lse2[b * p.hq + hq] = all;
+    lse2[b * p.hq + hq] = l > 0.f ? all : INFINITY;  // (+inf: every weight is 0)
     if (lse) lse[b * p.hq + hq] = l > 0.f ? all * kLn2 : -INFINITY;
   }
   const int streams = max(1, kRowThreads / p.d);  // head_dim <= 256

@@ -1,0 +1,36 @@
+"""Score and eviction calls at the edges of what they take."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from tests.test_scores_gpu import DEV, TDT, _case, _decode_wrapper  # noqa: E402
+
+
+@pytest.mark.parametrize("hq,hkv,d,ps,dtype", [(32, 8, 128, 16, "bfloat16"), (12, 3, 64, 16, "bfloat16"),
+                                               (14, 2, 64, 16, "float32"), (4, 2, 80, 16, "bfloat16"),
+                                               (16, 1, 64, 16, "bfloat16")])
+def test_decode_scores_of_rows_without_a_weight(hq, hkv, d, ps, dtype):
+    """Products that overflow to -inf for every token: such a head's output is 0
+    and its log-sum-exp -inf, and it gives no token a weight (NaN would stay in
+    the token's score for good)."""
+    c = _case(3, [40, 33], hq, hkv, d, ps, dtype)
+    c["t_pool"][:, 0, ..., 0] = torch.finfo(TDT[dtype]).max
+    q = torch.zeros(2, hq, d, dtype=TDT[dtype], device=DEV)
+    q[0, :, 0] = torch.finfo(TDT[dtype]).min    # request 0: every head
+    q[1, 1::2, 0] = torch.finfo(TDT[dtype]).min  # request 1: every other head
+    w = _decode_wrapper(c)
+    out, lse = w.run(q, c["t_pool"], return_lse=True, scores=c["t_scores"])
+    w.check_status()
+    dead = torch.zeros(2, hq, dtype=torch.bool, device=DEV)
+    dead[0], dead[1, 1::2] = True, True
+    assert torch.equal(lse == -np.inf, dead) and not out[dead].any()
+    got = c["t_scores"].double().cpu().numpy() - c["prior"]
+    group = hq // hkv
+    for b, n in enumerate((40, 33)):
+        pages = c["indices"][c["indptr"][b]:c["indptr"][b + 1]]
+        rows = got[pages].transpose(0, 2, 1).reshape(-1, hkv)[:n]
+        # q = 0: each live head gives each token 1 / n
+        live = [sum(not dead[b, h * group + g] for g in range(group)) for h in range(hkv)]
+        assert np.abs(rows - np.array([int(x) for x in live]) / n).max() <= 1e-6
