@@ -147,6 +147,8 @@ def evict_paged_kv_cache(paged_kv_cache: torch.Tensor, scores: torch.Tensor,
     if return_kept:
         shape = (batch, hkv, budget)
         kept = torch.empty((layers, *shape) if stacked else shape, dtype=torch.int32, device=dev)
+    if kv_indices.numel() == 0:  # no request holds a page
+        return kept.fill_(-1) if return_kept else None
     with on_device_of(paged_kv_cache):
         capi.call("mi_kv_evict", None, paged_kv_cache.data_ptr(),
                   paged_kv_cache.stride(0) if stacked else 0, scores.data_ptr(), layers,

@@ -5,7 +5,8 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from tests.test_scores_gpu import DEV, TDT, _case, _decode_wrapper  # noqa: E402
+from mi_b200.page import evict_paged_kv_cache  # noqa: E402
+from tests.test_scores_gpu import DEV, TDT, _case, _decode_wrapper, _i32  # noqa: E402
 
 
 @pytest.mark.parametrize("hq,hkv,d,ps,dtype", [(32, 8, 128, 16, "bfloat16"), (12, 3, 64, 16, "bfloat16"),
@@ -34,3 +35,13 @@ def test_decode_scores_of_rows_without_a_weight(hq, hkv, d, ps, dtype):
         # q = 0: each live head gives each token 1 / n
         live = [sum(not dead[b, h * group + g] for g in range(group)) for h in range(hkv)]
         assert np.abs(rows - np.array([int(x) for x in live]) / n).max() <= 1e-6
+
+
+def test_evict_without_pages():
+    """Requests that hold nothing at all: nothing to cut, nothing kept."""
+    kv = torch.ones(4, 2, 16, 2, 64, device=DEV, dtype=torch.bfloat16)
+    sc = torch.ones(4, 2, 16, device=DEV)
+    kept = evict_paged_kv_cache(kv, sc, _i32([]), _i32([0, 0, 0]), _i32([0, 0]), 8,
+                                return_kept=True)
+    assert kept.shape == (2, 2, 8) and (kept == -1).all()
+    assert (kv == 1).all() and (sc == 1).all()
