@@ -438,8 +438,11 @@ int mi_proj_small_m(const void *x, int64_t ldx, const void *w, int64_t ldw, cons
  * Each setting is per row (a device array of `rows`) or, where the array is
  * NULL, the scalar after it for all rows. logprob (optional): log-softmax of
  * the unscaled, unfiltered logits at the token. Deterministic (integer
- * masses); exact where two masses differ by more than about 2^-44 of the
- * likeliest token's. vocab <= 262144, no workspace. */
+ * masses). Each weight is exact to 2^-39 of itself and then to 2^-45 of the
+ * likeliest token's (held in steps of 2^-44): where a border of the filters or
+ * of the draw lies nearer to a running mass than that adds up to over the
+ * tokens before it, the token may fall on either side. vocab <= 262144, no
+ * workspace. */
 int mi_sample_tokens(const void *logits, int64_t row_stride, int32_t rows, int32_t vocab,
                      int32_t dtype, const float *uniform, const float *temperature,
                      float temperature_all, const int32_t *top_k, int32_t top_k_all,

@@ -10,10 +10,11 @@
 // All three filters keep a prefix of one total order, so a filter is a single
 // threshold on the composite (ordered key of x, ~index): what follows finds
 // that threshold without sorting the row. Weights are 45-bit fixed point (2^44
-// = the largest), computed in 64-bit floating point from the logit alone, and
-// summed as integers: sums are exact and the same in any order, so the result
-// does not depend on how the row is split or on the order of atomics, and a
-// near-flat row of 150,000 tokens still has 2^-44 of resolution per token.
+// = the largest), computed in 64-bit floating point from the logit alone (to
+// 2^-39 of themselves: the series of the exponential), and summed as integers:
+// sums are the same in any order, so the result does not depend on how the row
+// is split or on the order of atomics. The rounding to whole units is half a
+// unit a token: 2^-27 of the largest weight over 2^18 tokens at the most.
 //
 // One thread-block cluster per row (1 to 8 CTAs); each CTA keeps its slice of
 // the row in shared memory, read from HBM once. The passes exchange through

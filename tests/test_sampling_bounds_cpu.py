@@ -34,3 +34,19 @@ def test_eight_additions_reach_seven_roundings():
         s = np.float32(s + x)
     lost = v.sum() - float(s)
     assert 6.8 * 2.0 ** -24 * 0.98 < lost / v.sum() <= 7 * 2.0 ** -24
+
+
+def test_weights_are_exact_to_the_stated_2_to_the_minus_39():
+    """The kernel's weight, restated: 2^t from a table of 2^(j/32) and the series of
+    2^r to r^4, |r| <= 1/64. Its error is the series' rest, (r ln 2)^5 / 120."""
+    t = -np.random.default_rng(0).random(400_000) * 40
+    k = np.rint(t * 32)
+    r = t - k / 32
+    ln2 = math.log(2)
+    q = ((ln2 ** 4 / 24 * r + ln2 ** 3 / 6) * r + ln2 ** 2 / 2) * r + ln2
+    j = k.astype(np.int64)
+    w = np.ldexp(np.exp2((j & 31) / 32) * (1 + q * r), j >> 5)
+    want = np.exp2(t.astype(np.longdouble))
+    err = float(np.abs(w / want - 1).max())
+    assert err <= 2.0 ** -39
+    assert abs(err / ((ln2 / 64) ** 5 / 120) - 1) < 0.05  # (and no better than the series)
