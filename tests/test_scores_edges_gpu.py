@@ -6,6 +6,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 from mi_b200.page import evict_paged_kv_cache  # noqa: E402
+from mi_b200.prefill import BatchPrefillWithPagedKVCacheWrapper  # noqa: E402
 from tests.test_scores_gpu import DEV, TDT, _case, _decode_wrapper, _i32  # noqa: E402
 
 
@@ -45,3 +46,49 @@ def test_evict_without_pages():
                                 return_kept=True)
     assert kept.shape == (2, 2, 8) and (kept == -1).all()
     assert (kv == 1).all() and (sc == 1).all()
+
+
+def test_pages_past_32_bits():
+    """Pages whose rows lie past 2^32 bytes and 2^31 elements of the pool: the same
+    bits as in a small pool."""
+    hq, hkv, d, ps = 32, 8, 128, 16
+    c = _case(21, [300, 77], hq, hkv, d, ps, "bfloat16")
+    far = 140_000
+    kv = torch.empty(far + c["P"], 2, ps, hkv, d, dtype=torch.bfloat16, device=DEV)
+    assert far * 2 * ps * hkv * d > 2 ** 32
+    kv[far:] = c["t_pool"]
+    sc = torch.zeros(far + c["P"], hkv, ps, device=DEV)
+    sc[far:] = c["t_scores"]
+    q = torch.randn(2, hq, d, device=DEV, generator=torch.Generator(DEV).manual_seed(1)).bfloat16()
+    near = _decode_wrapper(c)
+    want = near.run(q, c["t_pool"], scores=c["t_scores"])
+    kept = evict_paged_kv_cache(c["t_pool"], c["t_scores"], c["t_indices"], c["t_indptr"],
+                                c["t_last"], 64, recent=9, sinks=2, return_kept=True)
+    c["t_indices"] = c["t_indices"] + far
+    got = _decode_wrapper(c).run(q, kv, scores=sc)
+    far_kept = evict_paged_kv_cache(kv, sc, c["t_indices"], c["t_indptr"], c["t_last"], 64,
+                                    recent=9, sinks=2, return_kept=True)
+    assert torch.equal(got, want) and torch.equal(far_kept, kept)
+    assert torch.equal(sc[far:], c["t_scores"]) and torch.equal(kv[far:], c["t_pool"])
+    assert not sc[:far].any()
+
+
+def test_prompt_scores_of_pages_past_32_bits():
+    hq, hkv, d, ps = 8, 8, 128, 16
+    for dtype in ("bfloat16", "float32"):
+        c = _case(22, [150], hq, hkv, d, ps, dtype)
+        far = 140_000 if dtype == "bfloat16" else 70_000
+        kv = torch.empty(far + c["P"], 2, ps, hkv, d, dtype=TDT[dtype], device=DEV)
+        kv[far:] = c["t_pool"]
+        sc = torch.zeros(far + c["P"], hkv, ps, device=DEV)
+        sc[far:] = c["t_scores"]
+        q = torch.randn(150, hq, d, device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+        q, lse = q.to(TDT[dtype]), torch.full((150, hq), 2.0, device=DEV)
+        w = BatchPrefillWithPagedKVCacheWrapper(torch.zeros(1 << 20, dtype=torch.uint8, device=DEV))
+        for pool, scores, base in ((c["t_pool"], c["t_scores"], 0), (kv, sc, far)):
+            w.plan(_i32([0, 150]), c["t_indptr"], c["t_indices"] + base, c["t_last"], hq, hkv, d,
+                   ps, causal=True)
+            w.accumulate_scores(q, pool, lse, scores, window=70)
+            w.check_status()
+        assert torch.equal(sc[far:], c["t_scores"]) and not sc[:far].any()
+        del kv, sc
