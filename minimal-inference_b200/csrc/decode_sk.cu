@@ -693,6 +693,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float p2 = exp2f(x2 - ms0), p3 = exp2f(x3 - ms0);
       l0 = l0 * corr0 + (p0 + p1 + p2 + p3);
       m0 = mn0;
+      // P in 16 bits for the product with V, as the instruction takes it: at most
+      // half a step (bf16 2^-8, fp16 2^-11) of each weight, an output by that share
+      // of its sum of w |v|; the row sum l0 and the stored logits keep 32 bits
       uint32_t pa[4];
       pa[0] = Mma<T>::pack(p0, p1);
       pa[2] = Mma<T>::pack(p2, p3);

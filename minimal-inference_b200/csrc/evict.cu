@@ -45,8 +45,8 @@ constexpr int kESmemMax = 200 * 1024;
 // KB of it static: 10360 tokens), that much: 64 requests of 8192 -> 8000 take 91
 // us, and 128 with the scores read again in each pass. Else (longer requests, or
 // a bound that says little, as a whole page table's) what leaves four CTAs' SM
-// 92 KB of L1, 6504 tokens: with 28 KB of L1 the rows' moves are slower (8 of up to
-// 4096 -> 1024 by their table's bound: 58 us for 48).
+// 92 KB of L1, 6504 tokens: with 28 KB of L1 the rows' moves are slower (8 of up
+// to 4096 -> 1024 by their table's bound: 58 us for 48).
 constexpr int kESmemFour = 43 * 1024;
 constexpr int kESmemSome = 27 * 1024;
 

@@ -6,8 +6,9 @@
 //
 // Two forms:
 //   * Decode (one query per request): the stream-K decode kernel already has
-//     every logit, so its score form stores them (fp32, log2 units; 1/16 of
-//     the bytes of K and V at 4 heads per KV head, and L2 resident) and
+//     every logit, so its score form stores them (fp32, log2 units; written and
+//     read back 8 bytes a token and query head, 1/16 of the bytes of K and V at
+//     4 heads of 128 per KV head, from L2 while a batch's fit it) and
 //     weights_kernel turns them into weights once the row sums are known:
 //     no second pass over K. fp32 and odd head sizes do the same in three
 //     plain kernels (logits by 16-token pieces, softmax and P V by row); other
