@@ -2,12 +2,15 @@
 import numpy as np
 import pytest
 
+from oracle import scores_oracle as so
+
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 from mi_b200.page import evict_paged_kv_cache  # noqa: E402
 from mi_b200.prefill import BatchPrefillWithPagedKVCacheWrapper  # noqa: E402
-from tests.test_scores_gpu import DEV, TDT, _case, _decode_wrapper, _i32  # noqa: E402
+from tests.test_scores_gpu import (DEV, TDT, _case, _check_scores, _decode_wrapper,  # noqa: E402
+                                   _expected, _i32, _mag, _prompt_check)
 
 
 @pytest.mark.parametrize("hq,hkv,d,ps,dtype", [(32, 8, 128, 16, "bfloat16"), (12, 3, 64, 16, "bfloat16"),
@@ -92,3 +95,22 @@ def test_prompt_scores_of_pages_past_32_bits():
             w.check_status()
         assert torch.equal(sc[far:], c["t_scores"]) and not sc[:far].any()
         del kv, sc
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(28, 4, 128, "bfloat16"), (14, 2, 64, "float32"),
+                                            (32, 32, 64, "float16")])
+def test_decode_scores_of_long_requests(hq, hkv, d, dtype):
+    lens = [20000, 1, 9001]
+    c = _case(40, lens, hq, hkv, d, 16, dtype)
+    q = torch.from_numpy(c["q"]).to(TDT[dtype]).to(DEV)
+    w = _decode_wrapper(c)
+    w.run(q, c["t_pool"], scores=c["t_scores"])
+    w.check_status()
+    add = _expected(c, lambda b, k: so.decode_weights(c["q"][b], k, d ** -0.5))
+    _check_scores(c, add, c["t_scores"], hq // hkv + max(lens) / 16, _mag(c["q"], c))
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(28, 4, 128, "bfloat16"), (14, 2, 64, "float32")])
+def test_prompt_scores_of_a_long_prompts_end(hq, hkv, d, dtype):
+    lens = [12000, 3, 5000]
+    _prompt_check(_case(41, lens, hq, hkv, d, 16, dtype), lens, [100, 3, 64], 64, True)
