@@ -49,9 +49,9 @@
 //
 // Bound by latency, not by its one read of the row: a row is a chain of
 // cluster barriers of 1-2 us with a few passes over shared memory between
-// them. Measured (CUDA graph): 12.5 us for 1 x 32768, 14 for 9 x 50257; 70
-// us for 64 x 152064 bf16 (nucleus of 0.9; the rows whose nucleus is wide take
-// 50 us of it), 121 us for 200 x 152064 fp32 with mixed settings (1.01 TB/s;
+// them. Measured (CUDA graph): 12.3 us for 1 x 32768, 13.4 for 9 x 50257; 70-75
+// us for 64 x 152064 bf16 (nucleus of 0.9, by the rows drawn; those whose nucleus
+// is wide take 50 us of it), 121 us for 200 x 152064 fp32 with mixed settings (1.01 TB/s;
 // clusters of 8 with two CTAs per SM pass in 5.4 waves).
 #include <cooperative_groups.h>
 
